@@ -2,7 +2,7 @@
  * Metal bridge (twally3/yue2_rs src/metal.m + src/attention.metal) on the
  * autoregressive single-token decode path.
  *
- * Two groups of entry points:
+ * Three groups of entry points:
  *
  *  1. Drop-ins for the Metal imports that src/tensor.rs:118-219 declares. Same
  *     argument lists and the same convention: 1 = done, 0 = not done. The reference
@@ -13,6 +13,9 @@
  *     sampling::generate (src/sampling.rs:222-294): weights, paged BF16 KV caches and
  *     the sampler state stay on the device and one decode step is one CUDA-graph
  *     launch. These return 0 on success or a negative YUE2_ERR_* code.
+ *
+ *  3. Operators over the caller's own device buffers: packed prompt attention, attention of
+ *     drafted tokens over paged K/V, the pass that writes the pages and the page moves.
  *
  * All pointers are host pointers unless stated. Calls on one Yue2Model (and the
  * caches/generators made from it) must not run concurrently; distinct models may be
@@ -343,6 +346,97 @@ void yue2_session_free(Yue2Session* ss);
  * of each other when the model uses them, as in the decode chain. Returns the mean launch time and
  * the weight bytes one launch streams. */
 int yue2_bench_gemv(Yue2Model* m, int kind, int rows, int launches, double* avg_ms, double* bytes);
+
+/* ================================================================== 3. operators
+ *
+ * Attention and cache operators over the caller's own device buffers, for hosts that keep
+ * their K/V in pages themselves (several requests of different lengths per call, prompts
+ * shared by several takes, drafted tokens checked in one pass). No counterpart in the
+ * reference, which serves one request at a time.
+ *
+ * Every pointer below is a device pointer of the current device (Yue2KvPool itself and the
+ * scalars are host values); `stream` is a cudaStream_t of that device (NULL: the default
+ * stream). The work is asynchronous on `stream`, nothing is allocated, and calls may be
+ * captured into CUDA graphs: lengths, page tables and lists are read on the device, so a
+ * replay may change their contents. Calls on different streams may overlap as long as their
+ * outputs and workspaces differ. The host checks sizes, strides, types and alignment and
+ * returns YUE2_ERR_INVALID before any launch. What only the device sees (page indexes,
+ * lengths, positions) is checked there: an entry out of range is skipped, so nothing outside
+ * the buffers is touched, and a YUE2_STATUS_* bit is set (atomic or) in `status`, one int32
+ * that the caller clears and reads when it likes.
+ *
+ * Vectors of one head are contiguous and the heads of a row adjacent; row strides are in
+ * elements, a multiple of 8, and every base is 16-byte aligned. Values are bf16 or f16. */
+#define YUE2_STATUS_PAGE 1  /* a page index or slot outside the pool */
+#define YUE2_STATUS_RANGE 2 /* a length, offset or position outside its buffer or table */
+#define YUE2_STATUS_STALL 4 /* a bounded device wait gave up: the call's outputs are invalid */
+
+/* Paged K/V: [pages][layers][K=0|V=1][kv][64 positions][dim], the layout of the library's own
+ * caches. Position p of a sequence lives in page table[p / 64], place p % 64; slot =
+ * 64 * page + place. dim is 64, 128 or 256 (64 or 128 for attention); dtype
+ * YUE2_DTYPE_BF16 or YUE2_DTYPE_F16. */
+typedef struct {
+  void* base;
+  uint64_t pages, layers, kv, dim;
+  int32_t dtype;
+} Yue2KvPool;
+
+/* RMSNorm of every q and k head (gains q_norm, k_norm [dim] f32, both NULL: no norm), the
+ * rotation of positions[row] (pairs (i, i + dim/2); cos and sin f32 [table_rows, dim/2]), and
+ * K and V written to slots[row] of the pool's `layer`, in one pass over the rows
+ * qkv [rows, heads + 2 kv, dim]. f32 throughout, one rounding. slots[row] < 0 writes no K/V;
+ * distinct rows have distinct slots. q_out [rows, heads, dim] and, when not NULL, k_out
+ * [rows, kv, dim] get the rotated heads; they may be the q and k parts of qkv itself (same
+ * base and stride). A row whose position is out of range is skipped whole. */
+int yue2_qk_rope_append(const void* qkv, uint64_t rows, uint64_t heads, uint64_t qkv_stride, const float* q_norm,
+                        const float* k_norm, float eps, const float* cos, const float* sin, uint64_t table_rows,
+                        const int32_t* positions, const Yue2KvPool* pool, uint64_t layer, const int64_t* slots,
+                        void* q_out, uint64_t q_stride, void* k_out, uint64_t k_stride, int32_t* status,
+                        void* stream);
+
+/* Attention over whole packed sequences: rows cu[s] .. cu[s+1] - 1 of q [tokens, heads, dim],
+ * k and v [tokens, kv, dim] are sequence s (cu: int32 [seqs + 1], nondecreasing, empty
+ * sequences allowed; at most 1,024 sequences and 262,144 tokens). A row sees the rows of its
+ * sequence up to itself (causal != 0) or all of them; out = softmax(scale q.k) v in `dtype`.
+ * Rows outside [cu[0], cu[seqs]) are neither read nor written, and what a masked position
+ * holds (infinities and NaN included) reaches no output. dim 64 or 128, heads a multiple of kv. */
+int yue2_attention_packed(const void* q, const void* k, const void* v, void* out, const int32_t* cu, uint64_t seqs,
+                          uint64_t tokens, uint64_t heads, uint64_t kv, uint64_t dim, uint64_t q_stride,
+                          uint64_t k_stride, uint64_t v_stride, uint64_t out_stride, int32_t dtype, int32_t causal,
+                          float scale, int32_t* status, void* stream);
+
+/* Attention of drafted tokens over the pages: sequence s (page table row table[s], table_pages
+ * entries) has context[s] positions and T = cu[s+1] - cu[s] <= 64 drafted ones after them,
+ * whose K/V are already in the pages (yue2_qk_rope_append). Row cu[s] + i of q [rows, heads,
+ * dim] sees the whole context and the drafted positions context[s] + j whose bit j is set in
+ * mask[cu[s] + i] (a node's ancestors and itself; bits >= T are ignored); mask NULL: j <= i,
+ * so T = 1 is an ordinary decode step. A row that sees nothing gets zeros; rows outside
+ * [cu[0], cu[seqs]) are left as they were. At most 1,024 sequences. `workspace`:
+ * yue2_attention_tree_workspace bytes (0: may be NULL), 16-byte aligned, contents free before
+ * and after; calls that may overlap need their own. */
+uint64_t yue2_attention_tree_workspace(uint64_t rows, uint64_t heads, uint64_t seqs, uint64_t table_pages,
+                                       const Yue2KvPool* pool);
+int yue2_attention_tree(const void* q, uint64_t rows, uint64_t heads, uint64_t q_stride, const Yue2KvPool* pool,
+                        uint64_t layer, const int32_t* table, uint64_t seqs, uint64_t table_pages,
+                        const int32_t* context, const int32_t* cu, const uint64_t* mask, float scale, void* out,
+                        uint64_t out_stride, void* workspace, uint64_t workspace_bytes, int32_t* status,
+                        void* stream);
+
+/* Positions [0, count[i]) (count NULL: all 64) of page src[i] to page dst[i], i < n, in every
+ * layer: what forking a sequence needs for its last, partly filled page (full pages are
+ * shared by their index). The dst pages are distinct and none of them is a src page. */
+int yue2_kv_copy(const Yue2KvPool* pool, const int32_t* src, const int32_t* dst, const int32_t* count, uint64_t n,
+                 int32_t* status, void* stream);
+
+/* Position keep[cu[s] + i] of sequence s to its position begin[s] + i, for i < cu[s+1] - cu[s],
+ * in every layer. dst_table NULL: in place, with keep strictly increasing and keep[cu[s]] >=
+ * begin[s] (accepting a path of a drafted tree, dropping positions); the pages of the
+ * positions written must belong to that sequence alone. Otherwise into the pages of
+ * dst_table [seqs, dst_pages], none of them a page that the call reads; keep in any order.
+ * `total` is the length of the list: cu[seqs] <= total. */
+int yue2_kv_gather(const Yue2KvPool* pool, const int32_t* src_table, uint64_t src_pages, const int32_t* dst_table,
+                   uint64_t dst_pages, const int32_t* begin, const int32_t* cu, const int32_t* keep, uint64_t seqs,
+                   uint64_t total, int32_t* status, void* stream);
 
 #ifdef __cplusplus
 }

@@ -72,6 +72,11 @@ class GpuLayer(ctypes.Structure):  # tensor.rs:231-237
     _fields_ = [("weights", GpuWeight * 7), ("norms", c_p * 4), ("key", c_p), ("value", c_p)]
 
 
+class KvPool(ctypes.Structure):
+    _fields_ = [("base", c_p), ("pages", c_u64), ("layers", c_u64), ("kv", c_u64), ("dim", c_u64),
+                ("dtype", ctypes.c_int32)]
+
+
 _PROTOS = {
     "yue2_last_error": (ctypes.c_char_p, []),
     "yue2_cuda_available": (c_int, []),
@@ -130,6 +135,15 @@ _PROTOS = {
     "yue2_session_free": (None, [c_p]),
     "yue2_bench_gemv": (c_int, [c_p, c_int, c_int, c_int, ctypes.POINTER(ctypes.c_double),
                                 ctypes.POINTER(ctypes.c_double)]),
+    "yue2_qk_rope_append": (c_int, [c_p, c_u64, c_u64, c_u64, c_p, c_p, c_f, c_p, c_p, c_u64, c_p, c_p, c_u64, c_p, c_p,
+                                    c_u64, c_p, c_u64, c_p, c_p]),
+    "yue2_attention_packed": (c_int, [c_p, c_p, c_p, c_p, c_p, c_u64, c_u64, c_u64, c_u64, c_u64, c_u64, c_u64, c_u64,
+                                      c_u64, ctypes.c_int32, ctypes.c_int32, c_f, c_p, c_p]),
+    "yue2_attention_tree_workspace": (c_u64, [c_u64, c_u64, c_u64, c_u64, c_p]),
+    "yue2_attention_tree": (c_int, [c_p, c_u64, c_u64, c_u64, c_p, c_u64, c_p, c_u64, c_u64, c_p, c_p, c_p, c_f, c_p,
+                                    c_u64, c_p, c_u64, c_p, c_p]),
+    "yue2_kv_copy": (c_int, [c_p, c_p, c_p, c_p, c_u64, c_p, c_p]),
+    "yue2_kv_gather": (c_int, [c_p, c_p, c_u64, c_p, c_u64, c_p, c_p, c_p, c_u64, c_u64, c_p, c_p]),
 }
 
 _lib = None

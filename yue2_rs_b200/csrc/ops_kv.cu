@@ -1,0 +1,293 @@
+// Operators that write the pages of a caller-owned K/V pool: QK norm + rotation + append,
+// page copies and position moves. All three are bound by HBM (every value read once and
+// written once); a page is [layers][K|V][kv] blocks of [64 positions][dim], so a position is
+// layers * 2 * kv separate runs of dim * 2 bytes.
+#include <string>
+
+#include "ops.cuh"
+
+namespace y2 {
+namespace {
+
+// ------------------------------------------------------------------ QK norm + rotation + append
+// y = x * rsqrt(mean(x^2) + eps) * gain, then (a, b) = (y_i, y_{i + D/2}) becomes
+// (a cos - b sin, b cos + a sin). One head is D/8 lanes of 8 elements (one 16-byte load and
+// store each); the partner i + D/2 of an element is D/16 lanes away, so a shuffle brings it.
+// One CTA per row: its groups of D/8 lanes take the row's heads in turn and keep the
+// row's cos and sin in registers.
+struct AppendParams {
+  const uint16_t* qkv;
+  uint16_t *q_out, *k_out;
+  const float *q_norm, *k_norm, *cos, *sin;
+  const int32_t* positions;
+  const int64_t* slots;
+  int32_t* status;
+  PoolView pool;
+  long long qkv_stride, q_stride, k_stride, table_rows;
+  int heads, layer;
+  float eps;
+};
+
+constexpr int kAppendThreads = 256;
+
+template <int D, bool F16>
+__global__ void __launch_bounds__(kAppendThreads) qk_rope_append_kernel(const AppendParams p) {
+  constexpr int L = D / 8;                     // lanes per head
+  constexpr int GROUPS = kAppendThreads / L;   // heads in flight
+  const long long row = blockIdx.x;
+  const int group = threadIdx.x / L, l = threadIdx.x % L;
+  const int kv = p.pool.kv, total = p.heads + 2 * kv;
+  const int pos = p.positions[row];
+  if (pos < 0 || pos >= p.table_rows) {
+    if (threadIdx.x == 0) status_or(p.status, YUE2_STATUS_RANGE);
+    return;
+  }
+  const long long slot = p.slots[row];
+  const bool store = slot >= 0 && (slot >> kPageLog2) < p.pool.pages;
+  if (slot >= 0 && !store && threadIdx.x == 0) status_or(p.status, YUE2_STATUS_PAGE);
+  uint16_t* page = p.pool.base + (store ? (slot >> kPageLog2) * p.pool.page_stride : 0);
+  const long long place = (slot & (kPageTokens - 1)) * D + l * 8;
+  const int half = (l % (L / 2)) * 8;
+  float c[8], s[8];
+  {
+    const float* ct = p.cos + (long long)pos * (D / 2) + half;
+    const float* st = p.sin + (long long)pos * (D / 2) + half;
+#pragma unroll
+    for (int e = 0; e < 8; e += 4) {
+      const float4 a = *reinterpret_cast<const float4*>(ct + e), b = *reinterpret_cast<const float4*>(st + e);
+      c[e] = a.x, c[e + 1] = a.y, c[e + 2] = a.z, c[e + 3] = a.w;
+      s[e] = b.x, s[e + 1] = b.y, s[e + 2] = b.z, s[e + 3] = b.w;
+    }
+  }
+  const uint16_t* src = p.qkv + row * p.qkv_stride + l * 8;
+  for (int h0 = 0; h0 < total; h0 += GROUPS) {
+    const int h = h0 + group;
+    const bool live = h < total;
+    const uint4 w = live ? *reinterpret_cast<const uint4*>(src + (long long)h * D) : make_uint4(0, 0, 0, 0);
+    float x[8];
+    unpack8<F16>(w, x);
+    const bool is_q = h < p.heads, is_v = h >= p.heads + kv;
+    if (p.q_norm) {
+      float ss = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
+#pragma unroll
+      for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      const float scale = 1.0f / sqrtf(ss / (float)D + p.eps);
+      const float* gain = (is_q ? p.q_norm : p.k_norm) + l * 8;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] *= scale * gain[e];
+    }
+    float y[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float other = __shfl_xor_sync(0xffffffffu, x[e], L / 2);
+      y[e] = l < L / 2 ? x[e] * c[e] - other * s[e] : x[e] * c[e] + other * s[e];
+    }
+    if (!live) continue;
+    const uint4 r = is_v ? w : pack8<F16>(y);
+    if (is_q) {
+      *reinterpret_cast<uint4*>(p.q_out + row * p.q_stride + (long long)h * D + l * 8) = r;
+    } else {
+      const int j = h - p.heads;  // K heads then V heads, as the pool's blocks of a layer
+      if (!is_v && p.k_out) *reinterpret_cast<uint4*>(p.k_out + row * p.k_stride + (long long)j * D + l * 8) = r;
+      if (store)
+        *reinterpret_cast<uint4*>(page + ((long long)p.layer * 2 * kv + j) * (kPageTokens * D) + place) = r;
+    }
+  }
+}
+
+// ------------------------------------------------------------------ page copy
+// CTA (block b, pair i): the first count[i] positions of one [64][dim] block, 16 KB at most.
+constexpr int kMoveThreads = 256;
+
+__global__ void __launch_bounds__(kMoveThreads) kv_copy_kernel(PoolView pool, const int32_t* src, const int32_t* dst,
+                                                               const int32_t* count, int32_t* status) {
+  const long long i = blockIdx.y;
+  const long long a = src[i], b = dst[i];
+  const int n = count ? count[i] : kPageTokens;
+  if (a < 0 || a >= pool.pages || b < 0 || b >= pool.pages || n < 0 || n > kPageTokens) {
+    if (threadIdx.x == 0 && blockIdx.x == 0)
+      status_or(status, n < 0 || n > kPageTokens ? YUE2_STATUS_RANGE : YUE2_STATUS_PAGE);
+    return;
+  }
+  const long long block = (long long)blockIdx.x * kPageTokens * pool.dim;
+  const uint4* from = reinterpret_cast<const uint4*>(pool.base + a * pool.page_stride + block);
+  uint4* to = reinterpret_cast<uint4*>(pool.base + b * pool.page_stride + block);
+  const int words = n * pool.dim / 8;
+  for (int w = threadIdx.x; w < words; w += kMoveThreads) to[w] = from[w];
+}
+
+// ------------------------------------------------------------------ position moves
+// CTA (block b, sequence s, share z): rows of dim * 2 bytes of one block, in chunks of
+// kMoveRows positions in list order. In place, keep is strictly increasing and keep[i] >= begin + i, so a
+// write of chunk c lands on positions that no later chunk reads; within a chunk every read
+// precedes every write (barrier). Out of place nothing read is written and the chunks of a
+// sequence go to several CTAs.
+struct GatherParams {
+  PoolView pool;
+  const int32_t *src_table, *dst_table, *begin, *cu, *keep;
+  int32_t* status;
+  long long src_pages, dst_pages, total;
+};
+
+template <int D>
+__global__ void __launch_bounds__(kMoveThreads) kv_gather_kernel(const GatherParams p) {
+  constexpr int L = D / 8;                     // lanes per row
+  constexpr int RP = kMoveThreads / L;         // rows per pass
+  constexpr int U = 4;                         // passes in flight
+  const int s = blockIdx.y;
+  const bool in_place = p.dst_table == nullptr;
+  const int first = p.cu[s], last = p.cu[s + 1], begin = p.begin[s];
+  const bool lead = threadIdx.x == 0 && blockIdx.x == 0;
+  if (first < 0 || last < first || last > p.total || begin < 0) {
+    if (lead && blockIdx.z == 0) status_or(p.status, YUE2_STATUS_RANGE);
+    return;
+  }
+  const int32_t* src_row = p.src_table + (long long)s * p.src_pages;
+  const int32_t* dst_row = in_place ? src_row : p.dst_table + (long long)s * p.dst_pages;
+  const long long dst_pages = in_place ? p.src_pages : p.dst_pages;
+  const long long block = (long long)blockIdx.x * kPageTokens * D;
+  const int sub = threadIdx.x / L, l = threadIdx.x % L;
+  const int n = last - first;
+  const int step = RP * U * gridDim.z;
+  for (int c0 = RP * U * blockIdx.z; c0 < n; c0 += step) {
+    uint4 v[U];
+    uint16_t* to[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = c0 + u * RP + sub;
+      to[u] = nullptr;
+      if (i >= n) continue;
+      const long long from = p.keep[first + i], dest = (long long)begin + i;
+      // the order that in-place moves rely on, for this entry and the one before it
+      const bool order = !in_place || (from >= dest && (i == 0 || p.keep[first + i - 1] < from));
+      if (from < 0 || (from >> kPageLog2) >= p.src_pages || (dest >> kPageLog2) >= dst_pages || !order) {
+        if (l == 0 && blockIdx.x == 0) status_or(p.status, YUE2_STATUS_RANGE);
+        continue;
+      }
+      const long long a = src_row[from >> kPageLog2], b = dst_row[dest >> kPageLog2];
+      if (a < 0 || a >= p.pool.pages || b < 0 || b >= p.pool.pages) {
+        if (l == 0 && blockIdx.x == 0) status_or(p.status, YUE2_STATUS_PAGE);
+        continue;
+      }
+      v[u] = *reinterpret_cast<const uint4*>(p.pool.base + a * p.pool.page_stride + block +
+                                             (from & (kPageTokens - 1)) * D + l * 8);
+      to[u] = p.pool.base + b * p.pool.page_stride + block + (dest & (kPageTokens - 1)) * D + l * 8;
+    }
+    if (in_place) __syncthreads();
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (to[u]) *reinterpret_cast<uint4*>(to[u]) = v[u];
+    if (in_place) __syncthreads();
+  }
+}
+
+}  // namespace
+}  // namespace y2
+
+using namespace y2;
+
+extern "C" {
+
+int yue2_qk_rope_append(const void* qkv, uint64_t rows, uint64_t heads, uint64_t qkv_stride, const float* q_norm,
+                        const float* k_norm, float eps, const float* cos, const float* sin, uint64_t table_rows,
+                        const int32_t* positions, const Yue2KvPool* pool, uint64_t layer, const int64_t* slots,
+                        void* q_out, uint64_t q_stride, void* k_out, uint64_t k_stride, int32_t* status,
+                        void* stream) {
+  AppendParams p = {};
+  int rc = check_pool(pool, false, p.pool);
+  if (rc || (rc = check_status(status))) return rc;
+  if (heads == 0 || heads > 1024 || rows > (uint64_t)INT32_MAX)
+    return fail(YUE2_ERR_INVALID, "heads must be in [1, 1024] and rows below 2^31");
+  if (layer >= pool->layers) return fail(YUE2_ERR_INVALID, "layer outside the KV pool");
+  if ((rc = check_rows(qkv, rows, heads + 2 * pool->kv, pool->dim, qkv_stride, "qkv"))) return rc;
+  if ((rc = check_rows(q_out, rows, heads, pool->dim, q_stride, "q_out"))) return rc;
+  if (k_out && (rc = check_rows(k_out, rows, pool->kv, pool->dim, k_stride, "k_out"))) return rc;
+  if (!q_norm != !k_norm) return fail(YUE2_ERR_INVALID, "q_norm and k_norm go together");
+  if (rows && (!positions || !slots || !cos || !sin || !aligned16(cos) || !aligned16(sin)))
+    return fail(YUE2_ERR_INVALID, "positions, slots and 16-byte aligned cos and sin tables are needed");
+  if (!(eps >= 0.f)) return fail(YUE2_ERR_INVALID, "eps must not be negative");
+  if (rows == 0) return 0;
+  p.qkv = (const uint16_t*)qkv;
+  p.q_out = (uint16_t*)q_out;
+  p.k_out = (uint16_t*)k_out;
+  p.q_norm = q_norm;
+  p.k_norm = k_norm;
+  p.cos = cos;
+  p.sin = sin;
+  p.positions = positions;
+  p.slots = slots;
+  p.status = status;
+  p.qkv_stride = (long long)qkv_stride;
+  p.q_stride = (long long)q_stride;
+  p.k_stride = (long long)k_stride;
+  p.table_rows = (long long)(table_rows < (uint64_t)INT64_MAX ? table_rows : INT64_MAX);
+  p.heads = (int)heads;
+  p.layer = (int)layer;
+  p.eps = eps;
+  const bool f16 = pool->dtype == YUE2_DTYPE_F16;
+  const dim3 grid((unsigned)rows);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+#define Y2_APPEND(DD)                                                              \
+  case DD:                                                                         \
+    if (f16) qk_rope_append_kernel<DD, true><<<grid, kAppendThreads, 0, st>>>(p);  \
+    else qk_rope_append_kernel<DD, false><<<grid, kAppendThreads, 0, st>>>(p);     \
+    break;
+  switch (p.pool.dim) {
+    Y2_APPEND(64)
+    Y2_APPEND(128)
+    Y2_APPEND(256)
+  }
+#undef Y2_APPEND
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? 0 : cuda_fail(e, "qk_rope_append launch");
+}
+
+int yue2_kv_copy(const Yue2KvPool* pool, const int32_t* src, const int32_t* dst, const int32_t* count, uint64_t n,
+                 int32_t* status, void* stream) {
+  PoolView v;
+  int rc = check_pool(pool, false, v);
+  if (rc || (rc = check_status(status))) return rc;
+  if (n > 65535) return fail(YUE2_ERR_INVALID, "at most 65,535 page pairs per call");
+  if (n && (!src || !dst)) return fail(YUE2_ERR_INVALID, "null page list");
+  if (n == 0) return 0;
+  kv_copy_kernel<<<dim3((unsigned)v.blocks, (unsigned)n), kMoveThreads, 0, static_cast<cudaStream_t>(stream)>>>(
+      v, src, dst, count, status);
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? 0 : cuda_fail(e, "kv_copy launch");
+}
+
+int yue2_kv_gather(const Yue2KvPool* pool, const int32_t* src_table, uint64_t src_pages, const int32_t* dst_table,
+                   uint64_t dst_pages, const int32_t* begin, const int32_t* cu, const int32_t* keep, uint64_t seqs,
+                   uint64_t total, int32_t* status, void* stream) {
+  GatherParams p = {};
+  int rc = check_pool(pool, false, p.pool);
+  if (rc || (rc = check_status(status))) return rc;
+  if (seqs > 65535 || total > (uint64_t)INT32_MAX || src_pages > (1u << 26) || dst_pages > (1u << 26))
+    return fail(YUE2_ERR_INVALID, "at most 65,535 sequences, 2^31 - 1 list entries and 2^26 pages per table row");
+  if (seqs == 0 || total == 0) return 0;
+  if (!src_table || !begin || !cu || !keep) return fail(YUE2_ERR_INVALID, "null table or list");
+  p.src_table = src_table;
+  p.dst_table = dst_table;
+  p.begin = begin;
+  p.cu = cu;
+  p.keep = keep;
+  p.status = status;
+  p.src_pages = (long long)src_pages;
+  p.dst_pages = (long long)dst_pages;
+  p.total = (long long)total;
+  // out of place: one CTA per 64 positions of the average list, at most 64 per (block, sequence)
+  const uint64_t shares = dst_table ? std::min<uint64_t>(64, (total / seqs + 63) / 64) : 1;
+  const dim3 grid((unsigned)p.pool.blocks, (unsigned)seqs, (unsigned)std::max<uint64_t>(1, shares));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  switch (p.pool.dim) {
+    case 64: kv_gather_kernel<64><<<grid, kMoveThreads, 0, st>>>(p); break;
+    case 128: kv_gather_kernel<128><<<grid, kMoveThreads, 0, st>>>(p); break;
+    case 256: kv_gather_kernel<256><<<grid, kMoveThreads, 0, st>>>(p); break;
+  }
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? 0 : cuda_fail(e, "kv_gather launch");
+}
+
+}  // extern "C"
