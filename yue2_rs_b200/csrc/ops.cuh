@@ -4,7 +4,9 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <cmath>
 #include <cstdint>
+#include <string>
 
 #include "../../include/yue2_cuda.h"
 #include "common.cuh"
@@ -89,6 +91,17 @@ inline int check_rows(const void* p, uint64_t rows, uint64_t heads, uint64_t dim
     return fail(YUE2_ERR_INVALID, std::string(what) + " must be a 16-byte aligned device pointer");
   if (stride % 8 || stride < heads * dim || stride > (1ull << 32))
     return fail(YUE2_ERR_INVALID, std::string(what) + ": the row stride must be a multiple of 8 that holds every head");
+  return 0;
+}
+
+inline int check_heads(uint64_t heads, uint64_t kv) {
+  if (heads == 0 || kv == 0 || heads > 1024 || kv > 1024 || heads % kv)
+    return fail(YUE2_ERR_INVALID, "heads must be a multiple of kv, both in [1, 1024]");
+  return 0;
+}
+
+inline int check_scale(float scale) {
+  if (!std::isfinite(scale)) return fail(YUE2_ERR_INVALID, "scale must be finite");
   return 0;
 }
 

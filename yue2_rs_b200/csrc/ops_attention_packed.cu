@@ -1,0 +1,441 @@
+// yue2_attention_packed: attention over whole packed sequences on the 5th-generation tensor
+// cores.
+//
+// A unit of work is 256 query rows of one head of one sequence: two sides of 128 rows that
+// share the stream of 128-key K and V tiles. Persistent CTAs (one per SM, 12 warps, two of them idle):
+//   warps 0-3, 4-7  softmax of side 0 and 1, thread = row = TMEM lane: scores from TMEM, weights
+//                   back to TMEM, the output at the end (softmax_tile in ops_tc.cuh);
+//   warp 8          one thread issues the products: while side 0's softmax runs, the tensor
+//                   cores do side 1's P.V and next scores, and the other way round;
+//   warp 9          picks the units, publishes them to the others and loads Q and the K, V ring by
+//                   TMA.
+// Units go out longest first (a causal unit's cost grows with its block), dealt to the CTAs
+// there and back (0..G-1, G-1..0, ..), found from the offsets on the device, so the host needs no
+// lengths. Heads of one block are neighbours, so that a group's K and V come from L2.
+#include <algorithm>
+#include <atomic>
+#include <cmath>
+
+#include "ops_tc.cuh"
+
+namespace y2 {
+namespace {
+
+using namespace opt;
+
+constexpr int kMaxSeqs = 1024;
+constexpr uint64_t kMaxTokens = 1u << 18;
+constexpr int kBlock = 2 * kRows;  // query rows of a unit
+constexpr int kUnits = 4;          // published units in flight
+
+struct PackedArgs {
+  const uint16_t* v;
+  uint16_t* out;
+  const int32_t* cu;
+  int32_t* status;
+  long long v_stride, out_stride;
+  int seqs, tokens, heads, group, causal, negate;
+  float c;  // |scale| log2(e)
+};
+
+struct Unit {
+  int first, n;     // the sequence's rows
+  int block, head;  // rows 256 * block .. of it; head < 0: no more units
+  int found;        // a value that is not finite was taken out of a masked tile
+};
+
+template <int D>
+struct Layout {
+  static constexpr int TILE = kRows * D * 2;  // bytes of a Q, K or V tile
+  static constexpr int SLOTS = D == 128 ? 5 : 8;
+  static constexpr int OFF_KV = 2 * TILE;
+  static constexpr int OFF_BAR = OFF_KV + SLOTS * TILE;
+  static constexpr int BARS = 2 * SLOTS + 2 * kUnits + 2 + 6 + 1;
+  static constexpr int OFF_UNIT = OFF_BAR + BARS * 8;
+  static constexpr int OFF_MISC = OFF_UNIT + kUnits * (int)sizeof(Unit);
+  static constexpr int BYTES = OFF_MISC + 16 + 1024;
+};
+
+struct Seq {
+  int first, n;
+};
+Y2_DEV Seq seq_of(const PackedArgs& a, int s) {
+  const int lo = a.cu[s], hi = a.cu[s + 1];
+  if (lo < 0 || hi < lo || hi > a.tokens) return {0, -1};
+  return {lo, hi - lo};
+}
+
+// The order of units (one warp): by block index from the highest down, within it by sequence
+// then head.
+struct Walk {
+  int level, base, count;
+};
+Y2_DEV int blocks_of(const PackedArgs& a, int s) {
+  return s < a.seqs ? (seq_of(a, s).n + kBlock - 1) / kBlock : 0;  // -1 rows: 0
+}
+Y2_DEV int count_above(const PackedArgs& a, int level) {
+  const int lane = threadIdx.x & 31;
+  int n = 0;
+  for (int s = 0; s < a.seqs; s += 32) n += __popc(__ballot_sync(0xffffffffu, blocks_of(a, s + lane) > level));
+  return n;
+}
+Y2_DEV void walk_begin(const PackedArgs& a, Walk& w) {
+  const int lane = threadIdx.x & 31;
+  int most = 0;
+  bool bad = false;
+  for (int s = lane; s < a.seqs; s += 32) {
+    bad |= seq_of(a, s).n < 0;
+    most = max(most, blocks_of(a, s));
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+  if (bad && blockIdx.x == 0) status_or(a.status, YUE2_STATUS_RANGE);
+  w.level = most - 1;
+  w.base = 0;
+  w.count = most > 0 ? count_above(a, w.level) : 0;
+}
+Y2_DEV Unit walk_to(const PackedArgs& a, Walk& w, int u) {
+  const int lane = threadIdx.x & 31;
+  while (w.level >= 0 && u >= w.base + w.count * a.heads) {
+    w.base += w.count * a.heads;
+    --w.level;
+    w.count = w.level >= 0 ? count_above(a, w.level) : 0;
+  }
+  Unit r = {0, 0, 0, -1, 0};
+  if (w.level < 0) return r;
+  int nth = (u - w.base) / a.heads;
+  const int head = (u - w.base) % a.heads;
+  for (int s = 0; s < a.seqs; s += 32) {
+    const uint32_t has = __ballot_sync(0xffffffffu, blocks_of(a, s + lane) > w.level);
+    if (nth < __popc(has)) {
+      const int at = s + __fns(has, 0, nth + 1);
+      const Seq q = seq_of(a, at);
+      r = {q.first, q.n, w.level, head, 0};
+      break;
+    }
+    nth -= __popc(has);
+  }
+  return r;
+}
+
+// Tiles of a side, and rows (0: the side has nothing to do).
+Y2_DEV int side_rows(const Unit& u, int side) { return max(0, min(kRows, u.n - u.block * kBlock - side * kRows)); }
+Y2_DEV int side_tiles(const PackedArgs& a, const Unit& u, int side) {
+  if (side_rows(u, side) == 0) return 0;
+  return a.causal ? 2 * u.block + side + 1 : (u.n + kKeys - 1) / kKeys;
+}
+
+template <int D, bool F16>
+__global__ void __launch_bounds__(kThreads, 1)
+    attention_packed_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
+                            const __grid_constant__ CUtensorMap mv, const PackedArgs a) {
+  using L = Layout<D>;
+  constexpr int SLOTS = L::SLOTS, TILE = L::TILE;
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint64_t* bar = (uint64_t*)(smem + L::OFF_BAR);
+  uint64_t *kv_full = bar, *kv_empty = bar + SLOTS, *unit_full = kv_empty + SLOTS, *unit_empty = unit_full + kUnits;
+  uint64_t *q_full = unit_empty + kUnits, *q_empty = q_full + 1, *s_full = q_empty + 1, *p_full = s_full + 2,
+           *o_full = p_full + 2, *drain = o_full + 2;
+  Unit* units = (Unit*)(smem + L::OFF_UNIT);
+  uint32_t* tmem_slot = (uint32_t*)(smem + L::OFF_MISC);
+  volatile int* ending = (volatile int*)(smem + L::OFF_MISC + 4);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < SLOTS; ++i) {
+      tc::mbar_init(kv_full + i, 1);
+      tc::mbar_init(kv_empty + i, 1);
+    }
+    for (int i = 0; i < kUnits; ++i) {
+      tc::mbar_init(unit_full + i, 1);
+      tc::mbar_init(unit_empty + i, 2 * kRows + 1);
+    }
+    tc::mbar_init(q_full, 1);
+    tc::mbar_init(q_empty, 1);
+    for (int i = 0; i < 2; ++i) {
+      tc::mbar_init(s_full + i, 1);
+      tc::mbar_init(p_full + i, kRows);
+      tc::mbar_init(o_full + i, 1);
+    }
+    tc::mbar_init(drain, 1);
+    *ending = 0;
+    tc::mbar_init_fence();
+  }
+  if (warp == 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(tmem_slot)),
+                 "r"(kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp >= 8) give_registers();
+  if (warp < 8) {
+    take_registers();
+    // ---------------------------------------------------------------- softmax and output
+    const int side = warp >> 2, t = threadIdx.x & (kRows - 1);
+    const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21);
+    const uint32_t s_addr = lanes + s_col(side), o_addr = lanes + o_col(side);
+    uint32_t s_phase = 0, o_phase = 0, kv_count = 0;
+    for (int k = 0;; ++k) {
+      const int us = k % kUnits;
+      if (!__all_sync(0xffffffffu, wait(unit_full + us, (k / kUnits) & 1, ending, a.status))) break;
+      const Unit u = units[us];
+      if (u.head < 0) break;
+      const int tiles = side_tiles(a, u, side), rows = side_rows(u, side);
+      const int row = u.block * kBlock + side * kRows + t;  // within the sequence
+      const int last = a.causal ? min(row, u.n - 1) : u.n - 1;
+      RowStats st = {-INFINITY, 0.f};
+      bool ok = true;
+      for (int j = 0; j < tiles; ++j) {
+        ok = __all_sync(0xffffffffu, wait(s_full + side, s_phase, ending, a.status));
+        if (!ok) break;
+        s_phase ^= 1;
+        tc::fence_after();
+        // only the last tile of a side has keys that some row does not see
+        const bool masked = j == tiles - 1 && (a.causal || u.n % kKeys);
+        uint32_t vis[4];
+        if (masked) {
+          const int seen = last - j * kKeys + 1;  // columns [0, seen)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int r = seen - 32 * q;
+            vis[q] = r >= 32 ? 0xffffffffu : r <= 0 ? 0u : (1u << r) - 1;
+          }
+        }
+        softmax_tile<D, F16>(s_addr, o_addr, a.c, a.negate, j == 0, masked, vis, st);
+        if (masked) {
+          const uint32_t at = kv_count + 2 * j + 1;
+          ok = __all_sync(0xffffffffu, wait(kv_full + at % SLOTS, (at / SLOTS) & 1, ending, a.status));
+          if (!ok) break;
+          if (clean_value_row<D, F16>(smem + L::OFF_KV + (at % SLOTS) * TILE, t, j * kKeys + t >= u.n)) units[us].found = 1;
+          tc::fence_proxy_async();
+        }
+        tc::fence_before();
+        tc::mbar_arrive(p_full + side);
+      }
+      if (!ok) break;
+      kv_count += 2 * max(side_tiles(a, u, 0), side_tiles(a, u, 1));
+      if (tiles) {
+        if (!__all_sync(0xffffffffu, wait(o_full + side, o_phase, ending, a.status))) break;
+        o_phase ^= 1;
+        tc::fence_after();
+        const float inv = 1.0f / st.l;
+        const bool found = *(volatile int*)&units[us].found;
+        uint16_t* dst = a.out + (long long)(u.first + row) * a.out_stride + u.head * D;
+#pragma unroll 1
+        for (int q = 0; q < D / 32; ++q) {
+          uint32_t o[32];
+          load32(o_addr + 32 * q, o);
+          wait_loads();
+          arrived(o);
+          float f[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(o[i]) * inv;
+          if (found && t < rows)  // keys of the unit's masked tiles that this row sees
+            for (int key = u.block * kBlock; key <= last; ++key)
+              add_nonfinite<F16>(a.v + (long long)(u.first + key) * a.v_stride + (u.head / a.group) * D + 32 * q, f);
+          if (t < rows) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 8) {
+              float x[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) x[e] = f[i + e];
+              *reinterpret_cast<uint4*>(dst + 32 * q + i) = pack8<F16>(x);
+            }
+          }
+        }
+        tc::fence_before();
+      }
+      tc::mbar_arrive(unit_empty + us);
+    }
+  } else if (warp == 8) {
+    // ---------------------------------------------------------------- products
+    if (lane == 0) {
+      const uint32_t qs = tc::smem_u32(smem), kvs = tc::smem_u32(smem + L::OFF_KV);
+      uint32_t p_phase[2] = {0, 0}, q_phase = 0, kv_count = 0;
+      auto kv_wait = [&](uint32_t at) { return wait(kv_full + at % SLOTS, (at / SLOTS) & 1, ending, a.status); };
+      auto kv_addr = [&](uint32_t at) { return kvs + (at % SLOTS) * TILE; };
+      bool ok = true;
+      for (int k = 0; ok; ++k) {
+        const int us = k % kUnits;
+        if (!(ok = wait(unit_full + us, (k / kUnits) & 1, ending, a.status))) break;
+        const Unit u = units[us];
+        if (u.head < 0) break;
+        const int tiles[2] = {side_tiles(a, u, 0), side_tiles(a, u, 1)}, all = max(tiles[0], tiles[1]);
+        if (!(ok = wait(q_full, q_phase, ending, a.status))) break;
+        q_phase ^= 1;
+        if (!(ok = kv_wait(kv_count))) break;
+        tc::fence_after();
+        for (int s = 0; s < 2; ++s)
+          if (tiles[s]) {
+            issue_scores<D, F16>(tmem + s_col(s), qs + s * TILE, kv_addr(kv_count));
+            tc::commit(s_full + s);
+          }
+        tc::commit(kv_empty + kv_count % SLOTS);
+        if (all == 1) tc::commit(q_empty);
+        for (int j = 0; j < all && ok; ++j) {
+          const uint32_t vt = kv_count + 2 * j + 1, kt = vt + 1;
+          if (!(ok = kv_wait(vt))) break;
+          if (j + 1 < all && !(ok = kv_wait(kt))) break;
+          for (int s = 0; s < 2; ++s) {
+            if (j >= tiles[s]) continue;
+            if (!(ok = wait(p_full + s, p_phase[s], ending, a.status))) break;
+            p_phase[s] ^= 1;
+            tc::fence_after();
+            issue_values<D, F16>(tmem + o_col(s), tmem + s_col(s), kv_addr(vt), j > 0);
+            if (j == tiles[s] - 1) {
+              tc::commit(o_full + s);
+            } else {
+              issue_scores<D, F16>(tmem + s_col(s), qs + s * TILE, kv_addr(kt));
+              tc::commit(s_full + s);
+            }
+          }
+          if (!ok) break;
+          tc::commit(kv_empty + vt % SLOTS);
+          if (j + 1 < all) tc::commit(kv_empty + kt % SLOTS);
+          if (j + 2 == all) tc::commit(q_empty);
+        }
+        if (!ok) break;
+        kv_count += 2 * all;
+        tc::mbar_arrive(unit_empty + us);
+      }
+      // every product is done before the TMEM goes (at once, unless a wait gave up)
+      tc::commit(drain);
+      settle(drain, 0, a.status);
+    }
+    __syncwarp();
+  } else if (warp == 9) {
+    // ---------------------------------------------------------------- units and loads
+    Walk w;
+    walk_begin(a, w);
+    uint32_t kv_count = 0, q_count = 0;
+    bool ok = true;
+    for (int k = 0; ok; ++k) {
+      const int g = (int)gridDim.x;
+      const Unit u = walk_to(a, w, k * g + (k & 1 ? g - 1 - (int)blockIdx.x : (int)blockIdx.x));
+      const int us = k % kUnits;
+      ok = __all_sync(0xffffffffu, wait(unit_empty + us, ((k / kUnits) & 1) ^ 1, ending, a.status));
+      if (!ok) break;
+      if (lane == 0) {
+        units[us] = u;
+        tc::mbar_arrive(unit_full + us);
+      }
+      __syncwarp();
+      if (u.head < 0) break;
+      const int both = side_rows(u, 1) > 0, all = max(side_tiles(a, u, 0), side_tiles(a, u, 1));
+      ok = __all_sync(0xffffffffu, wait(q_empty, (q_count & 1) ^ 1, ending, a.status));
+      if (!ok) break;
+      ++q_count;
+      const int row = u.first + u.block * kBlock, kvh = u.head / a.group;
+      if (lane == 0) {
+        tc::mbar_arrive_expect_tx(q_full, (both ? 2 : 1) * TILE);
+        for (int s = 0; s <= both; ++s)
+          for (int x = 0; x < D; x += 64)
+            tma_load_3d(smem + s * TILE + x / 64 * (kRows * 128), &mq, q_full, x, u.head, row + s * kRows);
+      }
+      for (int j = 0; j < 2 * all; ++j, ++kv_count) {
+        const int slot = kv_count % SLOTS;
+        ok = __all_sync(0xffffffffu, wait(kv_empty + slot, ((kv_count / SLOTS) & 1) ^ 1, ending, a.status));
+        if (!ok) break;
+        if (lane == 0) {
+          tc::mbar_arrive_expect_tx(kv_full + slot, TILE);
+          unsigned char* dst = smem + L::OFF_KV + slot * TILE;
+          for (int x = 0; x < D; x += 64)
+            tma_load_3d(dst + x / 64 * (kRows * 128), j & 1 ? &mv : &mk, kv_full + slot, x, kvh, u.first + (j >> 1) * kKeys);
+        }
+        __syncwarp();
+      }
+    }
+    // no copy in flight outlives the CTA (when a wait gave up, some may not have been used)
+    if (!ok) {
+      for (uint32_t i = kv_count > SLOTS ? kv_count - SLOTS : 0; i < kv_count; ++i)
+        settle(kv_full + i % SLOTS, (i / SLOTS) & 1, a.status);
+      if (q_count) settle(q_full, (q_count - 1) & 1, a.status);
+    }
+  }
+  tc::fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc::fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+  }
+}
+
+bool rows_map(CUtensorMap* m, const void* base, bool f16, uint64_t rows, uint64_t heads, uint64_t dim, uint64_t stride) {
+  const cuuint64_t dims[3] = {dim, heads, rows};
+  const cuuint64_t strides[2] = {dim * 2, stride * 2};
+  const cuuint32_t box[3] = {64, 1, (cuuint32_t)kRows}, step[3] = {1, 1, 1};
+  return cuTensorMapEncodeTiled(m, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+                                const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int D, bool F16>
+int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const PackedArgs& a, cudaStream_t st) {
+  int dev = 0, sms = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
+  e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaDeviceGetAttribute");
+  static std::atomic<uint64_t> ready{0};  // devices on which the shared-memory limit is set
+  if (dev >= 64 || !(ready.load(std::memory_order_relaxed) >> dev & 1)) {
+    e = cudaFuncSetAttribute(attention_packed_kernel<D, F16>, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<D>::BYTES);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute");
+    if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
+  }
+  const long long most = ((long long)a.tokens / kBlock + std::min(a.seqs, a.tokens)) * a.heads;
+  attention_packed_kernel<D, F16><<<(unsigned)std::min<long long>(sms, most), kThreads, Layout<D>::BYTES, st>>>(mq, mk, mv, a);
+  e = cudaGetLastError();
+  return e == cudaSuccess ? 0 : cuda_fail(e, "attention_packed launch");
+}
+
+}  // namespace
+}  // namespace y2
+
+using namespace y2;
+
+extern "C" int yue2_attention_packed(const void* q, const void* k, const void* v, void* out, const int32_t* cu,
+                                     uint64_t seqs, uint64_t tokens, uint64_t heads, uint64_t kv, uint64_t dim,
+                                     uint64_t q_stride, uint64_t k_stride, uint64_t v_stride, uint64_t out_stride,
+                                     int32_t dtype, int32_t causal, float scale, int32_t* status, void* stream) {
+  int rc = check_heads(heads, kv);
+  if (rc || (rc = check_status(status)) || (rc = check_scale(scale))) return rc;
+  if (dim != 64 && dim != 128) return fail(YUE2_ERR_INVALID, "attention takes a head dim of 64 or 128");
+  if (dtype != YUE2_DTYPE_BF16 && dtype != YUE2_DTYPE_F16) return fail(YUE2_ERR_INVALID, "values must be bf16 or f16");
+  if (seqs > (uint64_t)kMaxSeqs || tokens > kMaxTokens)
+    return fail(YUE2_ERR_INVALID, "at most 1,024 sequences and 262,144 tokens per call");
+  if ((rc = check_rows(q, tokens, heads, dim, q_stride, "q")) || (rc = check_rows(k, tokens, kv, dim, k_stride, "k")) ||
+      (rc = check_rows(v, tokens, kv, dim, v_stride, "v")) || (rc = check_rows(out, tokens, heads, dim, out_stride, "out")))
+    return rc;
+  if (seqs == 0 || tokens == 0) return 0;
+  if (!cu) return fail(YUE2_ERR_INVALID, "null sequence offsets");
+  const bool f16 = dtype == YUE2_DTYPE_F16;
+  CUtensorMap mq, mk, mv;
+  if (!rows_map(&mq, q, f16, tokens, heads, dim, q_stride) || !rows_map(&mk, k, f16, tokens, kv, dim, k_stride) ||
+      !rows_map(&mv, v, f16, tokens, kv, dim, v_stride))
+    return fail(YUE2_ERR_INVALID, "q, k or v cannot be described to the copy engine (base, strides)");
+  PackedArgs a = {};
+  a.v = (const uint16_t*)v;
+  a.out = (uint16_t*)out;
+  a.cu = cu;
+  a.status = status;
+  a.v_stride = (long long)v_stride;
+  a.out_stride = (long long)out_stride;
+  a.seqs = (int)seqs;
+  a.tokens = (int)tokens;
+  a.heads = (int)heads;
+  a.group = (int)(heads / kv);
+  a.causal = causal != 0;
+  a.negate = scale < 0.f;
+  // not below the smallest normal number: a masked score is -inf, and 0 * -inf is not 0
+  a.c = std::max(std::fabs(scale) * 1.4426950408889634f, 1.17549435e-38f);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (dim == 64) return f16 ? launch<64, true>(mq, mk, mv, a, st) : launch<64, false>(mq, mk, mv, a, st);
+  return f16 ? launch<128, true>(mq, mk, mv, a, st) : launch<128, false>(mq, mk, mv, a, st);
+}

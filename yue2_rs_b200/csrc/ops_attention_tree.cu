@@ -1,6 +1,6 @@
-// Attention operators over the caller's device buffers: whole packed prompts, and drafted
-// tokens over paged K/V. First form: one warp per (row, head) walks the visible keys with an
-// online softmax in f32; lanes hold D/32 elements of q and of the output.
+// yue2_attention_tree: attention of drafted tokens over paged K/V. First form: one warp per
+// (row, head) walks the visible keys with an online softmax in f32; lanes hold D/32 elements
+// of q and of the output.
 #include <cmath>
 #include <string>
 
@@ -10,7 +10,6 @@ namespace y2 {
 namespace {
 
 constexpr int kMaxSeqs = 1024;
-constexpr uint64_t kMaxTokens = 1u << 18;
 constexpr int kMaxNodes = 64;
 
 template <int D, bool F16>
@@ -50,16 +49,6 @@ struct RowState {
   }
 };
 
-struct PackedParams {
-  const uint16_t *q, *k, *v;
-  uint16_t* out;
-  const int32_t* cu;
-  int32_t* status;
-  long long q_stride, k_stride, v_stride, out_stride;
-  int seqs, tokens, heads, kv, causal;
-  float scale;
-};
-
 // The sequence that holds `row`, or -1. Offsets outside [0, rows] or decreasing are reported.
 Y2_DEV int find_seq(const int32_t* cu, int seqs, int rows, int row, int32_t* status) {
   int found = -1;
@@ -72,21 +61,6 @@ Y2_DEV int find_seq(const int32_t* cu, int seqs, int rows, int row, int32_t* sta
     if (row >= a && row < b && found < 0) found = s;
   }
   return found;
-}
-
-template <int D, bool F16>
-__global__ void __launch_bounds__(128) packed_kernel(const PackedParams p) {
-  const int row = blockIdx.x, lane = threadIdx.x & 31;
-  const int s = find_seq(p.cu, p.seqs, p.tokens, row, p.status);
-  if (s < 0) return;
-  const int first = p.cu[s], last = p.causal ? row : p.cu[s + 1] - 1;
-  for (int h = threadIdx.x >> 5; h < p.heads; h += 4) {
-    const long long at = (long long)(h / (p.heads / p.kv)) * D + lane * (D / 32);
-    RowState<D, F16> r;
-    r.begin(p.q + row * p.q_stride + h * D + lane * (D / 32));
-    for (int j = first; j <= last; ++j) r.key(p.k + j * p.k_stride + at, p.v + j * p.v_stride + at, p.scale);
-    r.end(p.out + row * p.out_stride + h * D + lane * (D / 32));
-  }
 }
 
 struct TreeParams {
@@ -134,55 +108,12 @@ __global__ void __launch_bounds__(128) tree_kernel(const TreeParams p) {
   }
 }
 
-int check_heads(uint64_t heads, uint64_t kv) {
-  if (heads == 0 || kv == 0 || heads > 1024 || kv > 1024 || heads % kv)
-    return fail(YUE2_ERR_INVALID, "heads must be a multiple of kv, both in [1, 1024]");
-  return 0;
-}
-
-int check_scale(float scale) {
-  if (!std::isfinite(scale)) return fail(YUE2_ERR_INVALID, "scale must be finite");
-  return 0;
-}
-
 }  // namespace
 }  // namespace y2
 
 using namespace y2;
 
 extern "C" {
-
-int yue2_attention_packed(const void* q, const void* k, const void* v, void* out, const int32_t* cu, uint64_t seqs,
-                          uint64_t tokens, uint64_t heads, uint64_t kv, uint64_t dim, uint64_t q_stride,
-                          uint64_t k_stride, uint64_t v_stride, uint64_t out_stride, int32_t dtype, int32_t causal,
-                          float scale, int32_t* status, void* stream) {
-  int rc = check_heads(heads, kv);
-  if (rc || (rc = check_status(status)) || (rc = check_scale(scale))) return rc;
-  if (dim != 64 && dim != 128) return fail(YUE2_ERR_INVALID, "attention takes a head dim of 64 or 128");
-  if (dtype != YUE2_DTYPE_BF16 && dtype != YUE2_DTYPE_F16) return fail(YUE2_ERR_INVALID, "values must be bf16 or f16");
-  if (seqs > (uint64_t)kMaxSeqs || tokens > kMaxTokens)
-    return fail(YUE2_ERR_INVALID, "at most 1,024 sequences and 262,144 tokens per call");
-  if ((rc = check_rows(q, tokens, heads, dim, q_stride, "q")) || (rc = check_rows(k, tokens, kv, dim, k_stride, "k")) ||
-      (rc = check_rows(v, tokens, kv, dim, v_stride, "v")) || (rc = check_rows(out, tokens, heads, dim, out_stride, "out")))
-    return rc;
-  if (seqs == 0 || tokens == 0) return 0;
-  if (!cu) return fail(YUE2_ERR_INVALID, "null sequence offsets");
-  PackedParams p = {(const uint16_t*)q, (const uint16_t*)k, (const uint16_t*)v, (uint16_t*)out, cu, status,
-                    (long long)q_stride, (long long)k_stride, (long long)v_stride, (long long)out_stride,
-                    (int)seqs, (int)tokens, (int)heads, (int)kv, causal != 0, scale};
-  const dim3 grid((unsigned)tokens);
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const bool f16 = dtype == YUE2_DTYPE_F16;
-  if (dim == 64) {
-    if (f16) packed_kernel<64, true><<<grid, 128, 0, st>>>(p);
-    else packed_kernel<64, false><<<grid, 128, 0, st>>>(p);
-  } else {
-    if (f16) packed_kernel<128, true><<<grid, 128, 0, st>>>(p);
-    else packed_kernel<128, false><<<grid, 128, 0, st>>>(p);
-  }
-  const cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? 0 : cuda_fail(e, "attention_packed launch");
-}
 
 uint64_t yue2_attention_tree_workspace(uint64_t, uint64_t, uint64_t, uint64_t, const Yue2KvPool*) { return 0; }
 
