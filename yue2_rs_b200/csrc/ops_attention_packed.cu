@@ -2,11 +2,15 @@
 // cores.
 //
 // A unit of work is 256 query rows of one head of one sequence: two sides of 128 rows that
-// share the stream of 128-key K and V tiles. Persistent CTAs (one per SM, 12 warps, two of them idle):
+// share the stream of 128-key K and V tiles. Persistent CTAs (one per SM, 10 warps):
 //   warps 0-3, 4-7  softmax of side 0 and 1, thread = row = TMEM lane: scores from TMEM, weights
 //                   back to TMEM, the output at the end (softmax_tile in ops_tc.cuh);
-//   warp 8          one thread issues the products: while side 0's softmax runs, the tensor
-//                   cores do side 1's P.V and next scores, and the other way round;
+//   warp 8          issues the products: while side 0's softmax runs, the tensor cores do side 1's
+//                   P.V and next scores, and the other way round (one warp for both keeps the
+//                   sides in turn: with a warp each they fell into step, both in softmax and
+//                   then both in products, a third slower). P.V starts when three quarters
+//                   of the weights are there, so that the last quarter's exponentials run
+//                   under it;
 //   warp 9          picks the units, publishes them to the others and loads Q and the K, V ring by
 //                   TMA.
 // Units go out longest first (a causal unit's cost grows with its block), dealt to the CTAs
@@ -25,6 +29,7 @@ using namespace opt;
 
 constexpr int kMaxSeqs = 1024;
 constexpr uint64_t kMaxTokens = 1u << 18;
+constexpr int kThreads = 320;
 constexpr int kBlock = 2 * kRows;  // query rows of a unit
 constexpr int kUnits = 4;          // published units in flight
 
@@ -50,7 +55,7 @@ struct Layout {
   static constexpr int SLOTS = D == 128 ? 5 : 8;
   static constexpr int OFF_KV = 2 * TILE;
   static constexpr int OFF_BAR = OFF_KV + SLOTS * TILE;
-  static constexpr int BARS = 2 * SLOTS + 2 * kUnits + 2 + 6 + 1;
+  static constexpr int BARS = 2 * SLOTS + 2 * kUnits + 2 + 8 + 1;
   static constexpr int OFF_UNIT = OFF_BAR + BARS * 8;
   static constexpr int OFF_MISC = OFF_UNIT + kUnits * (int)sizeof(Unit);
   static constexpr int BYTES = OFF_MISC + 16 + 1024;
@@ -118,7 +123,7 @@ Y2_DEV Unit walk_to(const PackedArgs& a, Walk& w, int u) {
   return r;
 }
 
-// Tiles of a side, and rows (0: the side has nothing to do).
+// Rows of a side (0: it has nothing to do), and its tiles of 128 keys.
 Y2_DEV int side_rows(const Unit& u, int side) { return max(0, min(kRows, u.n - u.block * kBlock - side * kRows)); }
 Y2_DEV int side_tiles(const PackedArgs& a, const Unit& u, int side) {
   if (side_rows(u, side) == 0) return 0;
@@ -135,8 +140,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint64_t* bar = (uint64_t*)(smem + L::OFF_BAR);
   uint64_t *kv_full = bar, *kv_empty = bar + SLOTS, *unit_full = kv_empty + SLOTS, *unit_empty = unit_full + kUnits;
-  uint64_t *q_full = unit_empty + kUnits, *q_empty = q_full + 1, *s_full = q_empty + 1, *p_full = s_full + 2,
-           *o_full = p_full + 2, *drain = o_full + 2;
+  uint64_t *q_full = unit_empty + kUnits, *q_empty = q_full + 1, *drain = q_empty + 1;
+  // per side: scores written, three quarters of the weights, all of them, the last P.V done
+  uint64_t *s_full = drain + 1, *p_part = s_full + 2, *p_full = p_part + 2, *o_full = p_full + 2;
   Unit* units = (Unit*)(smem + L::OFF_UNIT);
   uint32_t* tmem_slot = (uint32_t*)(smem + L::OFF_MISC);
   volatile int* ending = (volatile int*)(smem + L::OFF_MISC + 4);
@@ -149,16 +155,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int i = 0; i < kUnits; ++i) {
       tc::mbar_init(unit_full + i, 1);
-      tc::mbar_init(unit_empty + i, 2 * kRows + 1);
+      tc::mbar_init(unit_empty + i, 9);
     }
     tc::mbar_init(q_full, 1);
     tc::mbar_init(q_empty, 1);
+    tc::mbar_init(drain, 1);
     for (int i = 0; i < 2; ++i) {
       tc::mbar_init(s_full + i, 1);
-      tc::mbar_init(p_full + i, kRows);
+      tc::mbar_init(p_part + i, 4);
+      tc::mbar_init(p_full + i, 4);
       tc::mbar_init(o_full + i, 1);
     }
-    tc::mbar_init(drain, 1);
     *ending = 0;
     tc::mbar_init_fence();
   }
@@ -173,9 +180,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc::fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  if (warp >= 8) give_registers();
   if (warp < 8) {
-    take_registers();
     // ---------------------------------------------------------------- softmax and output
     const int side = warp >> 2, t = threadIdx.x & (kRows - 1);
     const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21);
@@ -189,34 +194,45 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int tiles = side_tiles(a, u, side), rows = side_rows(u, side);
       const int row = u.block * kBlock + side * kRows + t;  // within the sequence
       const int last = a.causal ? min(row, u.n - 1) : u.n - 1;
-      RowStats st = {-INFINITY, 0.f};
+      RowStats st;
+      st.begin();
       bool ok = true;
       for (int j = 0; j < tiles; ++j) {
         ok = __all_sync(0xffffffffu, wait(s_full + side, s_phase, ending, a.status));
         if (!ok) break;
         s_phase ^= 1;
         tc::fence_after();
-        // only the last tile of a side has keys that some row does not see
+        // the weights in TMEM so far, to the warp that issues the products: one arrival a warp
+        auto announce = [&](uint64_t* b) {
+          wait_stores();
+          tc::fence_before();
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive(b + side);
+        };
+        // only the last tile of a side has keys that some row does not see; the values of the
+        // last tile of either side are cleaned by both, whichever comes first
         const bool masked = j == tiles - 1 && (a.causal || u.n % kKeys);
+        const bool clean = masked || (a.causal && j == tiles - 1 - side);
+        const int seen = masked ? last - j * kKeys + 1 : kKeys;  // keys [0, seen) of the tile
         uint32_t vis[4];
-        if (masked) {
-          const int seen = last - j * kKeys + 1;  // columns [0, seen)
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int r = seen - 32 * q;
-            vis[q] = r >= 32 ? 0xffffffffu : r <= 0 ? 0u : (1u << r) - 1;
-          }
+        for (int q = 0; q < 4; ++q) {
+          const int r = seen - 32 * q;
+          vis[q] = r >= 32 ? 0xffffffffu : r <= 0 ? 0u : (1u << r) - 1;
         }
-        softmax_tile<D, F16>(s_addr, o_addr, a.c, a.negate, j == 0, masked, vis, st);
-        if (masked) {
+        if (clean) {
           const uint32_t at = kv_count + 2 * j + 1;
           ok = __all_sync(0xffffffffu, wait(kv_full + at % SLOTS, (at / SLOTS) & 1, ending, a.status));
           if (!ok) break;
-          if (clean_value_row<D, F16>(smem + L::OFF_KV + (at % SLOTS) * TILE, t, j * kKeys + t >= u.n)) units[us].found = 1;
+          for (int slab = 0; slab < D / 64; ++slab)
+            clean_values<F16>(smem + L::OFF_KV + (at % SLOTS) * TILE + slab * (kKeys * 128), t, j * kKeys + t >= u.n,
+                              &units[us].found);
           tc::fence_proxy_async();
         }
-        tc::fence_before();
-        tc::mbar_arrive(p_full + side);
+        auto part = [&] { announce(p_part); };
+        if (masked || a.negate) softmax_tile<D, F16, false>(s_addr, o_addr, a.c, a.negate, j == 0, vis, st, part);
+        else softmax_tile<D, F16, true>(s_addr, o_addr, a.c, false, j == 0, vis, st, part);
+        announce(p_full);
       }
       if (!ok) break;
       kv_count += 2 * max(side_tiles(a, u, 0), side_tiles(a, u, 1));
@@ -224,7 +240,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!__all_sync(0xffffffffu, wait(o_full + side, o_phase, ending, a.status))) break;
         o_phase ^= 1;
         tc::fence_after();
-        const float inv = 1.0f / st.l;
+        const float inv = 1.0f / st.total();
         const bool found = *(volatile int*)&units[us].found;
         uint16_t* dst = a.out + (long long)(u.first + row) * a.out_stride + u.head * D;
 #pragma unroll 1
@@ -251,65 +267,82 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         tc::fence_before();
       }
-      tc::mbar_arrive(unit_empty + us);
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(unit_empty + us);
     }
   } else if (warp == 8) {
     // ---------------------------------------------------------------- products
-    if (lane == 0) {
-      const uint32_t qs = tc::smem_u32(smem), kvs = tc::smem_u32(smem + L::OFF_KV);
-      uint32_t p_phase[2] = {0, 0}, q_phase = 0, kv_count = 0;
-      auto kv_wait = [&](uint32_t at) { return wait(kv_full + at % SLOTS, (at / SLOTS) & 1, ending, a.status); };
-      auto kv_addr = [&](uint32_t at) { return kvs + (at % SLOTS) * TILE; };
-      bool ok = true;
-      for (int k = 0; ok; ++k) {
-        const int us = k % kUnits;
-        if (!(ok = wait(unit_full + us, (k / kUnits) & 1, ending, a.status))) break;
-        const Unit u = units[us];
-        if (u.head < 0) break;
-        const int tiles[2] = {side_tiles(a, u, 0), side_tiles(a, u, 1)}, all = max(tiles[0], tiles[1]);
-        if (!(ok = wait(q_full, q_phase, ending, a.status))) break;
-        q_phase ^= 1;
-        if (!(ok = kv_wait(kv_count))) break;
-        tc::fence_after();
+    const uint32_t base = uniform(tmem), qs = tc::smem_u32(smem), kvs = tc::smem_u32(smem + L::OFF_KV);
+    uint32_t p_phase[2] = {0, 0}, q_phase = 0, kv_count = 0;
+    auto ready = [&](uint64_t* b, uint32_t parity) {
+      const bool r = __all_sync(0xffffffffu, wait(b, parity, ending, a.status)) != 0;
+      tc::fence_after();
+      return r;
+    };
+    auto kv_wait = [&](uint32_t at) { return ready(kv_full + at % SLOTS, (at / SLOTS) & 1); };
+    auto kv_addr = [&](uint32_t at) { return kvs + (at % SLOTS) * TILE; };
+    for (int k = 0;; ++k) {
+      const int us = k % kUnits;
+      if (!ready(unit_full + us, (k / kUnits) & 1)) break;
+      const Unit u = units[us];
+      if ((int)uniform(u.head) < 0) break;
+      const int tiles[2] = {(int)uniform(side_tiles(a, u, 0)), (int)uniform(side_tiles(a, u, 1))}, all = max(tiles[0], tiles[1]);
+      if (!ready(q_full, q_phase)) break;
+      q_phase ^= 1;
+      bool ok = kv_wait(kv_count);
+      if (!ok) break;
+      if (elect_one()) {
+#pragma unroll
         for (int s = 0; s < 2; ++s)
           if (tiles[s]) {
-            issue_scores<D, F16>(tmem + s_col(s), qs + s * TILE, kv_addr(kv_count));
+            issue_scores<D, F16>(base + s_col(s), qs + s * TILE, kv_addr(kv_count));
             tc::commit(s_full + s);
           }
         tc::commit(kv_empty + kv_count % SLOTS);
         if (all == 1) tc::commit(q_empty);
-        for (int j = 0; j < all && ok; ++j) {
-          const uint32_t vt = kv_count + 2 * j + 1, kt = vt + 1;
-          if (!(ok = kv_wait(vt))) break;
-          if (j + 1 < all && !(ok = kv_wait(kt))) break;
-          for (int s = 0; s < 2; ++s) {
-            if (j >= tiles[s]) continue;
-            if (!(ok = wait(p_full + s, p_phase[s], ending, a.status))) break;
-            p_phase[s] ^= 1;
-            tc::fence_after();
-            issue_values<D, F16>(tmem + o_col(s), tmem + s_col(s), kv_addr(vt), j > 0);
+      }
+      __syncwarp();
+      for (int j = 0; j < all; ++j) {
+        const uint32_t vt = kv_count + 2 * j + 1, kt = vt + 1;
+        ok = kv_wait(vt) && (j + 1 >= all || kv_wait(kt));
+        if (!ok) break;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          if (j >= tiles[s]) continue;
+          ok = ready(p_part + s, p_phase[s]);
+          if (!ok) break;
+          if (elect_one()) issue_values<D, F16>(base + o_col(s), base + s_col(s), kv_addr(vt), 0, 6, j > 0);
+          __syncwarp();
+          ok = ready(p_full + s, p_phase[s]);
+          if (!ok) break;
+          p_phase[s] ^= 1;
+          if (elect_one()) {
+            issue_values<D, F16>(base + o_col(s), base + s_col(s), kv_addr(vt), 6, 8, true);
             if (j == tiles[s] - 1) {
               tc::commit(o_full + s);
             } else {
-              issue_scores<D, F16>(tmem + s_col(s), qs + s * TILE, kv_addr(kt));
+              issue_scores<D, F16>(base + s_col(s), qs + s * TILE, kv_addr(kt));
               tc::commit(s_full + s);
             }
+            if (s == 1 || j >= tiles[1]) {  // the last side to use these tiles
+              tc::commit(kv_empty + vt % SLOTS);
+              if (j + 1 < all) tc::commit(kv_empty + kt % SLOTS);
+              if (j + 2 == all) tc::commit(q_empty);
+            }
           }
-          if (!ok) break;
-          tc::commit(kv_empty + vt % SLOTS);
-          if (j + 1 < all) tc::commit(kv_empty + kt % SLOTS);
-          if (j + 2 == all) tc::commit(q_empty);
+          __syncwarp();
         }
         if (!ok) break;
-        kv_count += 2 * all;
-        tc::mbar_arrive(unit_empty + us);
       }
-      // every product is done before the TMEM goes (at once, unless a wait gave up)
-      tc::commit(drain);
-      settle(drain, 0, a.status);
+      if (!ok) break;
+      kv_count += 2 * all;
+      if (lane == 0) tc::mbar_arrive(unit_empty + us);
     }
+    // every product is done before the TMEM goes (at once, unless a wait gave up)
+    if (elect_one()) tc::commit(drain);
     __syncwarp();
-  } else if (warp == 9) {
+    settle(drain, 0, a.status);
+  } else {
     // ---------------------------------------------------------------- units and loads
     Walk w;
     walk_begin(a, w);
@@ -327,7 +360,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       __syncwarp();
       if (u.head < 0) break;
-      const int both = side_rows(u, 1) > 0, all = max(side_tiles(a, u, 0), side_tiles(a, u, 1));
+      const int both = side_rows(u, 1) > 0, tiles = max(side_tiles(a, u, 0), side_tiles(a, u, 1));
       ok = __all_sync(0xffffffffu, wait(q_empty, (q_count & 1) ^ 1, ending, a.status));
       if (!ok) break;
       ++q_count;
@@ -338,7 +371,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int x = 0; x < D; x += 64)
             tma_load_3d(smem + s * TILE + x / 64 * (kRows * 128), &mq, q_full, x, u.head, row + s * kRows);
       }
-      for (int j = 0; j < 2 * all; ++j, ++kv_count) {
+      for (int j = 0; j < 2 * tiles; ++j, ++kv_count) {
         const int slot = kv_count % SLOTS;
         ok = __all_sync(0xffffffffu, wait(kv_empty + slot, ((kv_count / SLOTS) & 1) ^ 1, ending, a.status));
         if (!ok) break;

@@ -15,16 +15,10 @@ namespace y2 {
 namespace opt {
 
 constexpr int kRows = 128;   // query rows of a side
-constexpr int kKeys = 128;   // keys of a tile
+constexpr int kKeys = 128;   // keys of a K or V tile
 constexpr int kTmemCols = 512;
-__host__ __device__ constexpr int s_col(int side) { return 128 * side; }        // scores and probabilities
-__host__ __device__ constexpr int o_col(int side) { return 256 + 128 * side; }  // outputs
-// The block is launched with 12 warps of 168 registers (504 = 3 * 168 per lane of the three
-// warpgroups); the two softmax warpgroups hold a row of 128 scores and take more, the warps
-// that issue products and copies give theirs: 216 + 216 + 72 = 504.
-constexpr int kThreads = 384;
-Y2_DEV void take_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 216;"); }
-Y2_DEV void give_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 72;"); }
+__host__ __device__ constexpr int s_col(int side) { return 128 * side; }  // scores, then weights over them
+__host__ __device__ constexpr int o_col(int side) { return 256 + 128 * side; }
 constexpr long long kWaitCycles = 4000000000ll;  // about two seconds: a wait this long has failed
 
 // Waits for the phase of the given parity; false when the CTA is ending. A wait that lasts too
@@ -51,6 +45,19 @@ Y2_DEV void settle(uint64_t* bar, uint32_t parity, int32_t* status) {
     if (tc::mbar_try_wait(bar, parity)) return;
   status_or(status, YUE2_STATUS_STALL);
 }
+
+// One lane of the (converged) warp. The warp that issues products runs its control flow with all
+// lanes, so that descriptors stay in uniform registers, and only the instructions with one:
+// issued from a branch that one lane had taken, each product cost about 75 cycles.
+Y2_DEV bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\tselp.u32 %0, 1, 0, e;\n\t}"
+      : "=r"(p));
+  return p != 0;
+}
+// A value that every lane holds, for the compiler to know it.
+Y2_DEV uint32_t uniform(uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); }
 
 Y2_DEV void tma_load_3d(void* dst, const void* map, uint64_t* bar, int x, int y, int z) {
   asm volatile(
@@ -87,7 +94,8 @@ Y2_DEV void mma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t id
       : "memory");
 }
 
-// S = Q.K^T of one side: Q and K in slabs of [128 rows][64 dims].
+// S = Q.K^T of one side: Q and K in slabs of [128 rows][64 dims]. 128 keys a product: with 64
+// the reads of Q from shared memory (4 KB a product) would hold the tensor cores to 2/3.
 template <int D, bool F16>
 Y2_DEV void issue_scores(uint32_t tmem_s, uint32_t qs, uint32_t ks) {
 #pragma unroll
@@ -96,11 +104,11 @@ Y2_DEV void issue_scores(uint32_t tmem_s, uint32_t qs, uint32_t ks) {
     tc::mma_bf16(tmem_s, tc::sdesc_sw128(qs + off), tc::sdesc_sw128(ks + off), idesc<F16>(kKeys, false), kk > 0);
   }
 }
-// O (+)= P.V of one side.
+// O (+)= P.V of one side over the keys [16 k0, 16 k1) of a tile.
 template <int D, bool F16>
-Y2_DEV void issue_values(uint32_t tmem_o, uint32_t tmem_p, uint32_t vs, bool accumulate) {
+Y2_DEV void issue_values(uint32_t tmem_o, uint32_t tmem_p, uint32_t vs, int k0, int k1, bool accumulate) {
 #pragma unroll
-  for (int kk = 0; kk < kKeys / 16; ++kk)
+  for (int kk = k0; kk < k1; ++kk)
     mma_ts(tmem_o, tmem_p + kk * 8, vdesc(vs + kk * 2048), idesc<F16>(D, true), accumulate || kk > 0);
 }
 
@@ -135,6 +143,13 @@ Y2_DEV void store32(uint32_t taddr, const uint32_t (&v)[32]) {
       "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
       : "memory");
 }
+Y2_DEV void store16(uint32_t taddr, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
 Y2_DEV void wait_stores() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 Y2_DEV float ex2(float x) {
@@ -144,125 +159,199 @@ Y2_DEV float ex2(float x) {
 }
 
 // The running statistics of a thread's row: m is the score that the exponent is taken
-// relative to (not always the maximum so far, see below), l the sum of the weights.
+// relative to (not always the maximum so far, see softmax_tile), l the sum of the weights in parts.
 struct RowStats {
-  float m, l;
+  float m, l[4];
+  Y2_DEV void begin() { m = -INFINITY, l[0] = l[1] = l[2] = l[3] = 0.f; }
+  Y2_DEV float total() const { return (l[0] + l[1]) + (l[2] + l[3]); }
 };
 
-// One tile of a side's softmax: scores S in TMEM become weights p = 2^(c (s - m)), packed over
-// S, and l += sum p. c = |scale| log2(e), `negate` for a negative scale. With `masked`, bit i of `vis`
-// says whether the row sees key i of the tile. m moves, and O and l are scaled by 2^(c (m_old - m_new)),
-// only when a score exceeds it by more than a factor 2^8 of weight: until then the
-// weights are at most 2^8, exact in the f32 sums, and the final division by l removes the
-// factor; so most tiles leave O alone. p is rounded to 16 bits (relative error of half a
-// step, as the output's own rounding; l sums the unrounded weights). Every lane of the warp takes part.
-template <int D, bool F16>
-Y2_DEV void softmax_tile(uint32_t s_addr, uint32_t o_addr, float c, bool negate, bool first, bool masked,
-                         const uint32_t (&vis)[4], RowStats& st) {
-  uint32_t v[4][32];
-#pragma unroll
-  for (int q = 0; q < 4; ++q) load32(s_addr + 32 * q, v[q]);
-  wait_loads();
-#pragma unroll
-  for (int q = 0; q < 4; ++q) arrived(v[q]);
-  if (negate) {
-#pragma unroll
-    for (int q = 0; q < 4; ++q)
-#pragma unroll
-      for (int i = 0; i < 32; ++i) v[q][i] ^= 0x80000000u;
+// Pairs of f32 in one instruction.
+Y2_DEV void fma2(float& x, float& y, float ax, float ay, float bx, float by, float cx, float cy) {
+  asm("{\n\t.reg .b64 s, t, u;\n\t"
+      "mov.b64 s, {%2, %3};\n\tmov.b64 t, {%4, %5};\n\tmov.b64 u, {%6, %7};\n\t"
+      "fma.rn.f32x2 s, s, t, u;\n\tmov.b64 {%0, %1}, s;\n\t}"
+      : "=f"(x), "=f"(y)
+      : "f"(ax), "f"(ay), "f"(bx), "f"(by), "f"(cx), "f"(cy));
+}
+Y2_DEV void add2(float& x, float& y, float a, float b) {
+  asm("{\n\t.reg .b64 s, t;\n\t"
+      "mov.b64 s, {%0, %1};\n\tmov.b64 t, {%2, %3};\n\t"
+      "add.rn.f32x2 s, s, t;\n\tmov.b64 {%0, %1}, s;\n\t}"
+      : "+f"(x), "+f"(y)
+      : "f"(a), "f"(b));
+}
+
+// The largest of three, NaN if one of them is.
+Y2_DEV float max3(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// 2^x of two values on the FMA units: x = n + f with n the nearest integer and |f| <= 1/2, 2^f by
+// a polynomial fitted for the least relative error (degree 3 for bf16 weights: 7.5e-5, degree
+// 4 for f16: 2.6e-6; the rounding that follows is off by up to 3.9e-3 and 4.9e-4), and n added to its
+// exponent. x is below about 100 and not NaN; below -126 the result is 2^-126.
+template <bool F16>
+Y2_DEV void poly_ex2(float& x, float& y) {
+  constexpr float kRound = 12582912.f;  // 1.5 * 2^23: adding it leaves n in the low bits
+  x = fmaxf(x, -126.f);
+  y = fmaxf(y, -126.f);
+  float nx = x, ny = y;
+  add2(nx, ny, kRound, kRound);
+  float rx = nx, ry = ny;
+  add2(rx, ry, -kRound, -kRound);
+  float fx, fy, px, py;
+  fma2(fx, fy, rx, ry, -1.f, -1.f, x, y);
+  if constexpr (F16) {
+    fma2(px, py, 0x1.399776p-7f, 0x1.399776p-7f, fx, fy, 0x1.ca143ep-5f, 0x1.ca143ep-5f);
+    fma2(px, py, px, py, fx, fy, 0x1.ec06dcp-3f, 0x1.ec06dcp-3f);
+    fma2(px, py, px, py, fx, fy, 0x1.62e0dcp-1f, 0x1.62e0dcp-1f);
+    fma2(px, py, px, py, fx, fy, 0x1.ffffe8p-1f, 0x1.ffffe8p-1f);
+  } else {
+    fma2(px, py, 0x1.c3f694p-5f, 0x1.c3f694p-5f, fx, fy, 0x1.f0de16p-3f, 0x1.f0de16p-3f);
+    fma2(px, py, px, py, fx, fy, 0x1.62f31cp-1f, 0x1.62f31cp-1f);
+    fma2(px, py, px, py, fx, fy, 0x1.fff692p-1f, 0x1.fff692p-1f);
   }
-  if (masked) {
+  x = __uint_as_float(__float_as_uint(px) + (__float_as_uint(nx) << 23));
+  y = __uint_as_float(__float_as_uint(py) + (__float_as_uint(ny) << 23));
+}
+
+// 32 scores with the sign of the scale and without the keys that the row does not see. PLAIN:
+// a positive scale and every key seen. (Branches around the plain form would cut the code
+// into blocks across which loads, exponentials and products no longer overlap.)
+template <bool PLAIN>
+Y2_DEV void take_scores(uint32_t (&v)[32], bool negate, uint32_t vis) {
+  if constexpr (!PLAIN) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
-#pragma unroll
-      for (int i = 0; i < 32; ++i)
-        if (!(vis[q] >> i & 1)) v[q][i] = 0xff800000u;
+    for (int i = 0; i < 32; ++i) v[i] = vis >> i & 1 ? v[i] ^ (negate ? 0x80000000u : 0u) : 0xff800000u;
   }
-  float mx[4];
+}
+
+// A side's softmax over one tile of 128 keys: the scores in TMEM become weights
+// p = 2^(c (s - m)), packed over them. c = |scale| log2(e), `negate` for a negative scale; bit i of
+// `vis` says whether the row sees key i (both only without PLAIN). Every lane of the warp takes part.
+//
+// The maximum first. m starts as the first tile's and moves, O and l being scaled by
+// 2^(c (m_old - m_new)), only when a score exceeds it by more than a factor 2^8 of weight:
+// until then the weights are at most 2^8, exact in the f32 sums, and the final division by l
+// removes the factor. So most tiles leave O alone. O is settled: the P.V of the previous tile
+// was issued before the scores of this one. A score of +inf or NaN makes m so and the row NaN.
+//
+// Then the weights, in a second pass over the scores in TMEM (reading them again costs less
+// than holding 128 registers). p is rounded to 16 bits (relative error of half a step, as
+// the output's own rounding; l sums the unrounded weights). With PLAIN, kPoly of 16 pairs take the FMA
+// units, the others the special-function unit, which alone would need as long as the tensor
+// cores (8,192 rows of 24 heads: 787 us with 0, 764 with 2, 762 with 4, 759 with 8; masked keys need exact zeros). part() runs when 96 weights are stored; the caller announces the last 32.
+constexpr int kPoly = 4;
+template <int D, bool F16, bool PLAIN, class Part>
+Y2_DEV void softmax_tile(uint32_t s_addr, uint32_t o_addr, float c, bool negate, bool first, const uint32_t (&vis)[4],
+                         RowStats& st, Part part) {
+  uint32_t v[2][32];
+  float mx[4] = {st.m, st.m, st.m, st.m};
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    mx[q] = __uint_as_float(v[q][0]);
+  for (int h = 0; h < 2; ++h) {
+    load32(s_addr + 64 * h, v[0]);
+    load32(s_addr + 64 * h + 32, v[1]);
+    wait_loads();
+    arrived(v[0]);
+    arrived(v[1]);
+    take_scores<PLAIN>(v[0], negate, vis[2 * h]);
+    take_scores<PLAIN>(v[1], negate, vis[2 * h + 1]);
 #pragma unroll
-    for (int i = 1; i < 32; ++i) mx[q] = fmaxf(mx[q], __uint_as_float(v[q][i]));
+    for (int i = 0; i < 32; i += 4) {
+      mx[0] = max3(mx[0], __uint_as_float(v[0][i]), __uint_as_float(v[0][i + 1]));
+      mx[1] = max3(mx[1], __uint_as_float(v[0][i + 2]), __uint_as_float(v[0][i + 3]));
+      mx[2] = max3(mx[2], __uint_as_float(v[1][i]), __uint_as_float(v[1][i + 1]));
+      mx[3] = max3(mx[3], __uint_as_float(v[1][i + 2]), __uint_as_float(v[1][i + 3]));
+    }
   }
-  const float mn = fmaxf(st.m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
-  const bool move = first || (mn - st.m) * c > 8.0f;
+  load32(s_addr, v[0]);
+  const float mn = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]);
+  const bool move = first || !((mn - st.m) * c <= 8.0f);  // NaN moves too
   if (!first && __any_sync(0xffffffffu, move)) {
     const float alpha = move ? ex2((st.m - mn) * c) : 1.0f;
-    st.l *= alpha;
 #pragma unroll
-    for (int q = 0; q < D / 32; ++q) {
-      uint32_t o[32];
-      load32(o_addr + 32 * q, o);
-      wait_loads();
-      arrived(o);
+    for (int i = 0; i < 4; ++i) st.l[i] *= alpha;
+#pragma unroll 1
+    for (int q = 0; q < D; q += 16) {
+      uint32_t o[16];
+      tc::tmem_ld16(o_addr + q, o);
 #pragma unroll
-      for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-      store32(o_addr + 32 * q, o);
+      for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+      store16(o_addr + q, o);
     }
   }
   if (move) st.m = mn;
-  const float mc = st.m == -INFINITY ? 0.f : st.m * c;
-  float sum[4] = {0.f, 0.f, 0.f, 0.f};
-  uint32_t p[2][32];
+  const float mc = st.m == -INFINITY ? 0.f : st.m == INFINITY ? NAN : -st.m * c;
 #pragma unroll
-  for (int q = 0; q < 4; ++q)
+  for (int q = 0; q < 4; ++q) {
+    uint32_t(&s)[32] = v[q & 1];
+    wait_loads();
+    arrived(s);
+    if (q < 3) load32(s_addr + 32 * (q + 1), v[(q + 1) & 1]);
+    take_scores<PLAIN>(s, negate, vis[q]);
+    uint32_t p[16];
 #pragma unroll
-    for (int i = 0; i < 32; i += 2) {
-      const float a = ex2(fmaf(__uint_as_float(v[q][i]), c, -mc)), b = ex2(fmaf(__uint_as_float(v[q][i + 1]), c, -mc));
-      sum[q] += a;
-      sum[q] += b;
-      p[q >> 1][(q & 1) * 16 + i / 2] = pack16<F16>(a, b);
+    for (int i = 0; i < 16; ++i) {
+      float a, b;
+      fma2(a, b, __uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]), c, c, mc, mc);
+      if (PLAIN && i % (16 / kPoly) == 16 / kPoly - 1) {
+        poly_ex2<F16>(a, b);
+      } else {
+        a = ex2(a);
+        b = ex2(b);
+      }
+      add2(st.l[2 * (i & 1)], st.l[2 * (i & 1) + 1], a, b);
+      p[i] = pack16<F16>(a, b);
     }
-  st.l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-  store32(s_addr, p[0]);
-  store32(s_addr + 32, p[1]);
-  wait_stores();
+    store16(s_addr + 16 * q, p);
+    if (q == 2) part();
+  }
 }
 
-// Key `r` of a V tile in shared memory (slabs of [128][64 dims], 128-byte swizzle) where some
-// row of the tile does not see it: a value that is not finite would reach those rows as
-// 0 * inf, so it becomes zero here, and true is returned for the rows that do see it to add
-// it at the end. dead: no row sees the key, all of it becomes zero.
-template <int D, bool F16>
-Y2_DEV bool clean_value_row(unsigned char* vs, int r, bool dead) {
+// Key `r` of a V tile in shared memory (slabs of [128][64 dims], 128-byte swizzle), 64 dims of
+// it (slab at `vs`), where some row of the side does not see it: a value that is not finite
+// would reach those rows as 0 * inf, so it becomes zero here, and *found is set (before, for who
+// reads the zero) for the rows that do see it to add it at the end. dead: no row sees the
+// key, all of it becomes zero.
+template <bool F16>
+Y2_DEV void clean_values(unsigned char* vs, int r, bool dead, int* found) {
   constexpr uint32_t EXP = F16 ? 0x7c00u : 0x7f80u;
-  bool found = false;
 #pragma unroll
-  for (int s = 0; s < D / 64; ++s)
-#pragma unroll
-    for (int ch = 0; ch < 8; ++ch) {
-      uint4* at = reinterpret_cast<uint4*>(vs + s * (kKeys * 128) + tc::sw128(r, ch));
-      if (dead) {
-        *at = make_uint4(0, 0, 0, 0);
-        continue;
-      }
-      uint4 w = *at;
-      uint32_t* x = reinterpret_cast<uint32_t*>(&w);
-      bool bad = false;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if ((x[i] & EXP) == EXP) x[i] &= 0xffff0000u, bad = true;
-        if ((x[i] >> 16 & EXP) == EXP) x[i] &= 0x0000ffffu, bad = true;
-      }
-      if (bad) *at = w, found = true;
+  for (int ch = 0; ch < 8; ++ch) {
+    uint4* at = reinterpret_cast<uint4*>(vs + tc::sw128(r, ch));
+    if (dead) {
+      *at = make_uint4(0, 0, 0, 0);
+      continue;
     }
-  return found;
+    uint4 w = *at;
+    uint32_t* x = reinterpret_cast<uint32_t*>(&w);
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if ((x[i] & EXP) == EXP) x[i] &= 0xffff0000u, bad = true;
+      if ((x[i] >> 16 & EXP) == EXP) x[i] &= 0x0000ffffu, bad = true;
+    }
+    if (bad) {
+      *(volatile int*)found = 1;
+      __threadfence_block();
+      *at = w;
+    }
+  }
 }
 
 // Adds the values of a key that are not finite (32 of them at `v`) to a row's outputs.
 template <bool F16>
 Y2_DEV void add_nonfinite(const uint16_t* v, float (&o)[32]) {
+#pragma unroll
   for (int i = 0; i < 32; i += 8) {
     float x[8];
     unpack8<F16>(*reinterpret_cast<const uint4*>(v + i), x);
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      if (!isfinite(x[e])) {
-#pragma unroll
-        for (int k = 0; k < 32; k += 8)
-          if (k == i) o[k + e] += x[e];
-      }
+      if (!isfinite(x[e])) o[i + e] += x[e];
   }
 }
 
