@@ -399,16 +399,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-bool rows_map(CUtensorMap* m, const void* base, bool f16, uint64_t rows, uint64_t heads, uint64_t dim, uint64_t stride) {
-  const cuuint64_t dims[3] = {dim, heads, rows};
-  const cuuint64_t strides[2] = {dim * 2, stride * 2};
-  const cuuint32_t box[3] = {64, 1, (cuuint32_t)kRows}, step[3] = {1, 1, 1};
-  return cuTensorMapEncodeTiled(m, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
-                                const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <int D, bool F16>
 int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const PackedArgs& a, cudaStream_t st) {
   int dev = 0, sms = 0;
@@ -450,8 +440,9 @@ extern "C" int yue2_attention_packed(const void* q, const void* k, const void* v
   if (!cu) return fail(YUE2_ERR_INVALID, "null sequence offsets");
   const bool f16 = dtype == YUE2_DTYPE_F16;
   CUtensorMap mq, mk, mv;
-  if (!rows_map(&mq, q, f16, tokens, heads, dim, q_stride) || !rows_map(&mk, k, f16, tokens, kv, dim, k_stride) ||
-      !rows_map(&mv, v, f16, tokens, kv, dim, v_stride))
+  if (!opt::make_rows_map(&mq, f16, q, tokens, heads, dim, q_stride, 1, opt::kRows) ||
+      !opt::make_rows_map(&mk, f16, k, tokens, kv, dim, k_stride, 1, opt::kRows) ||
+      !opt::make_rows_map(&mv, f16, v, tokens, kv, dim, v_stride, 1, opt::kRows))
     return fail(YUE2_ERR_INVALID, "q, k or v cannot be described to the copy engine (base, strides)");
   PackedArgs a = {};
   a.v = (const uint16_t*)v;

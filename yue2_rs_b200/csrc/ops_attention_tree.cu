@@ -1,111 +1,636 @@
-// yue2_attention_tree: attention of drafted tokens over paged K/V. First form: one warp per
-// (row, head) walks the visible keys with an online softmax in f32; lanes hold D/32 elements
-// of q and of the output.
+// yue2_attention_tree: attention of drafted tokens over paged K/V on the 5th-generation tensor
+// cores, bound by reading the pages.
+//
+// The G = heads / kv query heads of a group share K and V, so a tile has rows (node, head): 128
+// of them are a side (floor(128 / G) nodes). An item of work is one kv head of one
+// sequence with up to two sides of rows; its keys come in tiles of 128 (two pages). When the
+// rows fill one side, both sides hold them and take the tiles in turn, and their results are
+// merged in TMEM: two softmax warps then keep up with HBM even when a single warp has rows.
+//
+// The tiles of all items form one line, cut into equal shares for the CTAs (one per SM), so
+// that one long context among short ones loads every SM alike. An item cut between CTAs
+// leaves partial results (output, maximum and sum, f32) that a second kernel merges in tile
+// order; items that lie in one share are finished at once. The shares follow from the
+// lengths on the device, so the host needs none of them.
+//
+// A CTA is ten warps as in attention_packed: softmax of the sides, products, page loads (TMA).
+#include <algorithm>
+#include <atomic>
 #include <cmath>
-#include <string>
 
-#include "ops.cuh"
+#include "ops_tc.cuh"
 
 namespace y2 {
 namespace {
 
+using namespace opt;
+
 constexpr int kMaxSeqs = 1024;
 constexpr int kMaxNodes = 64;
+constexpr int kMaxGroup = 128;  // query heads per kv head: one node's rows fit a side
+constexpr int kThreads = 320;
+constexpr int kUnits = 4;
+constexpr int kMergeThreads = 256;
 
-template <int D, bool F16>
-struct RowState {
-  static constexpr int DL = D / 32;
-  float q[DL], o[DL], m = -INFINITY, l = 0.f;
-  Y2_DEV static void load(const uint16_t* p, float (&v)[DL]) {
-#pragma unroll
-    for (int e = 0; e < DL; e += 2) {
-      const uint32_t w = *reinterpret_cast<const uint32_t*>(p + e);
-      v[e] = lo16<F16>(w), v[e + 1] = hi16<F16>(w);
-    }
-  }
-  Y2_DEV void begin(const uint16_t* p) {
-    load(p, q);
-#pragma unroll
-    for (int e = 0; e < DL; ++e) o[e] = 0.f;
-  }
-  Y2_DEV void key(const uint16_t* kp, const uint16_t* vp, float scale) {
-    float k[DL], v[DL], s = 0.f;
-    load(kp, k);
-    load(vp, v);
-#pragma unroll
-    for (int e = 0; e < DL; ++e) s = fmaf(q[e], k[e], s);
-    s = warp_sum(s) * scale;
-    const float mn = fmaxf(m, s);
-    const float a = m == -INFINITY ? 0.f : expf(m - mn), w = expf(s - mn);
-    m = mn;
-    l = l * a + w;
-#pragma unroll
-    for (int e = 0; e < DL; ++e) o[e] = fmaf(w, v[e], o[e] * a);
-  }
-  Y2_DEV void end(uint16_t* p) {
-    const float inv = l > 0.f ? 1.0f / l : l == 0.f ? 0.f : l;
-#pragma unroll
-    for (int e = 0; e < DL; e += 2) *reinterpret_cast<uint32_t*>(p + e) = pack16<F16>(o[e] * inv, o[e + 1] * inv);
-  }
-};
-
-// The sequence that holds `row`, or -1. Offsets outside [0, rows] or decreasing are reported.
-Y2_DEV int find_seq(const int32_t* cu, int seqs, int rows, int row, int32_t* status) {
-  int found = -1;
-  for (int s = 0; s < seqs; ++s) {
-    const int a = cu[s], b = cu[s + 1];
-    if (a < 0 || b < a || b > rows) {
-      status_or(status, YUE2_STATUS_RANGE);
-      continue;
-    }
-    if (row >= a && row < b && found < 0) found = s;
-  }
-  return found;
-}
-
-struct TreeParams {
-  const uint16_t* q;
+struct TreeArgs {
   uint16_t* out;
-  PoolView pool;
+  const uint16_t* pool;
   const int32_t *table, *context, *cu;
   const uint64_t* mask;
   int32_t* status;
-  long long q_stride, out_stride, table_pages;
-  int seqs, rows, heads, layer;
-  float scale;
+  float* part;  // [2 * CTAs][slot_rows][D] outputs, then [2 * CTAs][slot_rows][2] maximum and sum
+  long long out_stride, pages, page_stride, table_pages;
+  int seqs, rows, heads, kv, group, nodes, layer, blocks, negate, ctas, slot_rows;
+  float c;  // |scale| log2(e)
 };
 
+// One sequence: rows first .. first + n - 1, its context, tiles of 128 keys and row blocks of
+// up to 2 * a.nodes nodes. n = 0: nothing to do. A bad entry is reported once.
+struct SeqWork {
+  int first, n, tiles, parts;
+  long long ctx;
+};
+Y2_DEV SeqWork seq_work(const TreeArgs& a, int s, bool report) {
+  SeqWork w = {0, 0, 0, 0, 0};
+  const int lo = a.cu[s], hi = a.cu[s + 1], ctx = a.context[s];
+  if (lo < 0 || hi < lo || hi > a.rows || hi - lo > kMaxNodes || ctx < 0 ||
+      (hi > lo && (long long)ctx + hi - lo > a.table_pages * kPageTokens)) {
+    if (report) status_or(a.status, YUE2_STATUS_RANGE);
+    return w;
+  }
+  if (hi == lo) return w;
+  w.first = lo;
+  w.n = hi - lo;
+  w.ctx = ctx;
+  w.tiles = (int)((w.ctx + w.n + kKeys - 1) / kKeys);
+  w.parts = (w.n + 2 * a.nodes - 1) / (2 * a.nodes);
+  return w;
+}
+Y2_DEV long long seq_tiles(const TreeArgs& a, const SeqWork& w) { return (long long)w.tiles * w.parts * a.kv; }
+
+// Shares: CTA c of `used` takes tiles [share(c), share(c + 1)) of `all`.
+Y2_DEV int used_ctas(const TreeArgs& a, long long all) { return (int)min((long long)a.ctas, max(all, 1ll)); }
+Y2_DEV long long share(long long all, int used, int c) { return all * c / used; }
+// The CTA whose share holds tile x.
+Y2_DEV int owner(long long all, int used, long long x) {
+  int c = (int)(x * used / all);
+  while (share(all, used, c) > x) --c;
+  while (share(all, used, c + 1) <= x) ++c;
+  return c;
+}
+
+struct Unit {
+  int first, n, node, head;  // the sequence's rows, the block's first node, the kv head (< 0: end)
+  int seq, t0, t1;           // tiles [t0, t1)
+  int slot;                  // partial results to this slot; < 0: the item is complete
+  long long ctx;
+  int found;
+};
+
+template <int D>
+struct Layout {
+  static constexpr int TILE = kRows * D * 2;
+  static constexpr int SLOTS = D == 128 ? 5 : 8;
+  static constexpr int OFF_KV = 2 * TILE;
+  static constexpr int OFF_BAR = OFF_KV + SLOTS * TILE;
+  static constexpr int BARS = 2 * SLOTS + 2 * kUnits + 2 + 1 + 8 + 2;
+  static constexpr int OFF_UNIT = OFF_BAR + BARS * 8;
+  static constexpr int OFF_ML = OFF_UNIT + kUnits * (int)sizeof(Unit);
+  static constexpr int OFF_MISC = OFF_ML + kRows * 8;
+  static constexpr int BYTES = OFF_MISC + 16 + 1024;
+};
+
+// A unit's sides. One side of nodes: both hold it and side s takes tiles t0 + s, t0 + s + 2, ..
+Y2_DEV bool in_turn(const TreeArgs& a, const Unit& u) { return u.n - u.node <= a.nodes; }
+Y2_DEV int side_tiles(const TreeArgs& a, const Unit& u, int side) {
+  const int t = u.t1 - u.t0;
+  return in_turn(a, u) ? (t + 1 - side) / 2 : t;
+}
+
+// Bits [p, p + 32) of what a node sees: the context, then its mask over the n drafted positions.
+Y2_DEV uint32_t seen_bits(long long p, long long ctx, uint64_t mask) {
+  const long long sh = p - ctx;
+  if (sh >= 64) return 0;
+  if (sh >= 0) return (uint32_t)(mask >> sh);
+  if (sh <= -32) return 0xffffffffu;
+  return (uint32_t)(mask << -sh) | ((1u << -sh) - 1);
+}
+
 template <int D, bool F16>
-__global__ void __launch_bounds__(128) tree_kernel(const TreeParams p) {
-  const int row = blockIdx.x, lane = threadIdx.x & 31;
-  const int s = find_seq(p.cu, p.seqs, p.rows, row, p.status);
-  if (s < 0) return;
-  const int i = row - p.cu[s], nodes = p.cu[s + 1] - p.cu[s];
-  const long long ctx = p.context[s];
-  if (nodes > kMaxNodes || ctx < 0 || ctx + nodes > p.table_pages * kPageTokens) {
-    status_or(p.status, YUE2_STATUS_RANGE);
-    return;
-  }
-  const int32_t* table = p.table + s * p.table_pages;
-  const uint64_t mask = p.mask ? p.mask[row] : ~0ull >> (63 - i);
-  for (int h = threadIdx.x >> 5; h < p.heads; h += 4) {
-    const int g = h / (p.heads / p.pool.kv);
-    RowState<D, F16> r;
-    r.begin(p.q + row * p.q_stride + h * D + lane * (D / 32));
-    for (long long j = 0; j < ctx + nodes; ++j) {
-      if (j >= ctx && !(mask >> (j - ctx) & 1)) continue;
-      const long long page = table[j >> kPageLog2];
-      if (page < 0 || page >= p.pool.pages) {
-        status_or(p.status, YUE2_STATUS_PAGE);
-        continue;
-      }
-      const uint16_t* kp = p.pool.base + page * p.pool.page_stride +
-                           ((long long)(p.layer * 2) * p.pool.kv + g) * (kPageTokens * D) +
-                           (j & (kPageTokens - 1)) * D + lane * (D / 32);
-      r.key(kp, kp + (long long)p.pool.kv * (kPageTokens * D), p.scale);
+__global__ void __launch_bounds__(kThreads, 1)
+    attention_tree_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mkv, const TreeArgs a) {
+  using L = Layout<D>;
+  constexpr int SLOTS = L::SLOTS, TILE = L::TILE;
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint64_t* bar = (uint64_t*)(smem + L::OFF_BAR);
+  uint64_t *kv_full = bar, *kv_empty = bar + SLOTS, *unit_full = kv_empty + SLOTS, *unit_empty = unit_full + kUnits;
+  uint64_t *q_full = unit_empty + kUnits, *q_empty = q_full + 1, *drain = q_empty + 1;
+  // per side: scores written, three quarters of the weights, all of them, the last P.V done
+  uint64_t *s_full = drain + 1, *p_part = s_full + 2, *p_full = p_part + 2, *o_full = p_full + 2;
+  uint64_t *ml_full = o_full + 2, *ml_empty = ml_full + 1;  // side 1's statistics, for the merge
+  Unit* units = (Unit*)(smem + L::OFF_UNIT);
+  float2* ml = (float2*)(smem + L::OFF_ML);
+  uint32_t* tmem_slot = (uint32_t*)(smem + L::OFF_MISC);
+  volatile int* ending = (volatile int*)(smem + L::OFF_MISC + 4);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < SLOTS; ++i) {
+      tc::mbar_init(kv_full + i, 1);
+      tc::mbar_init(kv_empty + i, 1);
     }
-    r.end(p.out + row * p.out_stride + h * D + lane * (D / 32));
+    for (int i = 0; i < kUnits; ++i) {
+      tc::mbar_init(unit_full + i, 1);
+      tc::mbar_init(unit_empty + i, 9);
+    }
+    tc::mbar_init(q_full, 1);
+    tc::mbar_init(q_empty, 1);
+    tc::mbar_init(drain, 1);
+    for (int i = 0; i < 2; ++i) {
+      tc::mbar_init(s_full + i, 1);
+      tc::mbar_init(p_part + i, 4);
+      tc::mbar_init(p_full + i, 4);
+      tc::mbar_init(o_full + i, 1);
+    }
+    tc::mbar_init(ml_full, 4);
+    tc::mbar_init(ml_empty, 4);
+    *ending = 0;
+    tc::mbar_init_fence();
   }
+  if (warp == 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(tmem_slot)),
+                 "r"(kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_trigger();  // the merge may be set up meanwhile; it waits for this grid's results
+
+  if (warp < 8) {
+    // ---------------------------------------------------------------- softmax and output
+    const int side = warp >> 2, t = threadIdx.x & (kRows - 1);
+    const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21);
+    const uint32_t s_addr = lanes + s_col(side), o_addr = lanes + o_col(side);
+    uint32_t s_phase = 0, o_phase = 0, ml_phase = 0, kv_count = 0;
+    for (int k = 0;; ++k) {
+      const int us = k % kUnits;
+      if (!__all_sync(0xffffffffu, wait(unit_full + us, (k / kUnits) & 1, ending, a.status))) break;
+      const Unit u = units[us];
+      if (u.head < 0) break;
+      const bool turns = in_turn(a, u);
+      const int tiles = side_tiles(a, u, side), stride = turns ? 2 : 1;
+      const int node0 = u.node + (turns ? 0 : side * a.nodes);
+      const int rows = min(a.nodes, u.n - node0) * a.group;
+      const int node = node0 + t / a.group;  // of the sequence
+      const bool live = t < rows, warp_live = (warp & 3) * 32 < rows;
+      const uint64_t drafted = u.n < 64 ? (1ull << u.n) - 1 : ~0ull;
+      uint64_t mask = 0;
+      if (live) mask = a.mask ? a.mask[u.first + node] & drafted : (node < 63 ? (2ull << node) - 1 : ~0ull);
+      RowStats st;
+      st.begin();
+      bool ok = true;
+      for (int i = 0; i < tiles; ++i) {
+        const int j = u.t0 + (turns ? side : 0) + i * stride;  // tile of the sequence
+        ok = __all_sync(0xffffffffu, wait(s_full + side, s_phase, ending, a.status));
+        if (!ok) break;
+        s_phase ^= 1;
+        tc::fence_after();
+        auto announce = [&](uint64_t* b) {
+          wait_stores();
+          tc::fence_before();
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive(b + side);
+        };
+        auto part = [&] { announce(p_part); };
+        const long long key0 = (long long)j * kKeys;
+        const bool masked = key0 + kKeys > u.ctx;  // the tile reaches into the drafted positions
+        if (masked) {
+          const uint32_t at = kv_count + 2 * (j - u.t0) + 1;
+          ok = __all_sync(0xffffffffu, wait(kv_full + at % SLOTS, (at / SLOTS) & 1, ending, a.status));
+          if (!ok) break;
+          if (key0 + t >= u.ctx)
+            for (int slab = 0; slab < D / 64; ++slab)
+              clean_values<F16>(smem + L::OFF_KV + (at % SLOTS) * TILE + slab * (kKeys * 128), t, key0 + t >= u.ctx + u.n,
+                                &units[us].found);
+          tc::fence_proxy_async();
+        }
+        if (!warp_live) {
+          part();
+        } else if (masked || a.negate) {
+          uint32_t vis[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) vis[q] = seen_bits(key0 + 32 * q, u.ctx, mask);
+          softmax_tile<D, F16, false>(s_addr, o_addr, a.c, a.negate, i == 0, vis, st, part);
+        } else {
+          const uint32_t vis[4] = {};
+          softmax_tile<D, F16, true>(s_addr, o_addr, a.c, false, i == 0, vis, st, part);
+        }
+        announce(p_full);
+      }
+      if (!ok) break;
+      kv_count += 2 * (u.t1 - u.t0);
+      if (tiles) {
+        ok = __all_sync(0xffffffffu, wait(o_full + side, o_phase, ending, a.status));
+        if (!ok) break;
+        o_phase ^= 1;
+        tc::fence_after();
+      }
+      // the two sides of one set of rows: side 1 hands over its statistics, side 0 reads both outputs
+      const bool merge = turns && u.t1 - u.t0 > 1;
+      float l = st.total(), w0 = 1.f, w1 = 0.f, m = st.m;
+      if (merge && side == 1) {
+        ml[t] = make_float2(st.m, l);
+        tc::fence_before();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(ml_full);
+        ok = __all_sync(0xffffffffu, wait(ml_empty, ml_phase, ending, a.status));
+        if (!ok) break;
+        ml_phase ^= 1;
+        tc::fence_after();
+      } else if (merge) {
+        ok = __all_sync(0xffffffffu, wait(ml_full, ml_phase, ending, a.status));
+        if (!ok) break;
+        ml_phase ^= 1;
+        tc::fence_after();
+        const float2 o = ml[t];
+        m = max3(m, o.x, o.x);
+        if (m != -INFINITY) {
+          w0 = st.m == -INFINITY ? 0.f : ex2((st.m - m) * a.c);
+          w1 = o.x == -INFINITY ? 0.f : ex2((o.x - m) * a.c);
+        }
+        l = l * w0 + o.y * w1;
+      }
+      if (warp_live && (side == 0 || !turns)) {
+        const bool found = *(volatile int*)&units[us].found;
+        const float inv = l > 0.f ? 1.0f / l : l == 0.f ? 0.f : l;  // nothing seen: zeros
+        const int row = u.first + node, head = u.head * a.group + t % a.group;
+        uint16_t* dst = a.out + (long long)row * a.out_stride + (long long)head * D;
+        const long long prow = (long long)u.slot * a.slot_rows + (node - u.node) * a.group + t % a.group;
+#pragma unroll 1
+        for (int q = 0; q < D / 32; ++q) {
+          uint32_t o[32];
+          load32(o_addr + 32 * q, o);
+          wait_loads();
+          arrived(o);
+          float f[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) f[i] = w0 == 0.f ? 0.f : __uint_as_float(o[i]) * w0;
+          if (merge) {
+            load32(lanes + o_col(1) + 32 * q, o);
+            wait_loads();
+            arrived(o);
+            if (w1 != 0.f) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) f[i] = fmaf(__uint_as_float(o[i]), w1, f[i]);
+            }
+          }
+          if (found && live) {  // drafted values that are not finite, of the keys of these tiles
+            for (int d = 0; d < u.n; ++d) {
+              const long long key = u.ctx + d;
+              if (!(mask >> d & 1) || key < (long long)u.t0 * kKeys || key >= (long long)u.t1 * kKeys) continue;
+              const long long page = a.table[(long long)u.seq * a.table_pages + (key >> kPageLog2)];
+              if (page < 0 || page >= a.pages) continue;
+              add_nonfinite<F16>(a.pool + page * a.page_stride +
+                                     ((long long)(a.layer * 2 + 1) * a.kv + u.head) * (kPageTokens * D) +
+                                     (key & (kPageTokens - 1)) * D + 32 * q,
+                                 f);
+            }
+          }
+          if (!live) continue;
+          if (u.slot >= 0) {
+            float4* p = reinterpret_cast<float4*>(a.part + prow * D + 32 * q);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) p[i] = make_float4(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; i += 8) {
+              float x[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) x[e] = f[i + e] * inv;
+              *reinterpret_cast<uint4*>(dst + 32 * q + i) = pack8<F16>(x);
+            }
+          }
+        }
+        if (live && u.slot >= 0)
+          reinterpret_cast<float2*>(a.part + 2ll * a.ctas * a.slot_rows * D)[prow] = make_float2(m, l);
+      }
+      tc::fence_before();
+      __syncwarp();
+      if (merge && side == 0 && lane == 0) tc::mbar_arrive(ml_empty);
+      if (lane == 0) tc::mbar_arrive(unit_empty + us);
+    }
+  } else if (warp == 8) {
+    // ---------------------------------------------------------------- products
+    const uint32_t base = uniform(tmem), qs = tc::smem_u32(smem), kvs = tc::smem_u32(smem + L::OFF_KV);
+    uint32_t p_phase[2] = {0, 0}, q_phase = 0, kv_count = 0;
+    auto ready = [&](uint64_t* b, uint32_t parity) {
+      const bool r = __all_sync(0xffffffffu, wait(b, parity, ending, a.status)) != 0;
+      tc::fence_after();
+      return r;
+    };
+    auto kv_wait = [&](uint32_t at) { return ready(kv_full + at % SLOTS, (at / SLOTS) & 1); };
+    auto kv_addr = [&](uint32_t at) { return kvs + (at % SLOTS) * TILE; };
+    for (int k = 0;; ++k) {
+      const int us = k % kUnits;
+      if (!ready(unit_full + us, (k / kUnits) & 1)) break;
+      const Unit u = units[us];
+      if ((int)uniform(u.head) < 0) break;
+      const bool turns = uniform(in_turn(a, u)) != 0;
+      const int all = (int)uniform(u.t1 - u.t0);
+      if (!ready(q_full, q_phase)) break;
+      q_phase ^= 1;
+      // the first scores of both sides: of tile 0, or of tiles 0 and 1 in turn
+      const int firsts = turns ? min(all, 2) : 1;
+      bool ok = true;
+      for (int j = 0; j < firsts && ok; ++j) {
+        ok = kv_wait(kv_count + 2 * j);
+        if (!ok) break;
+        if (elect_one()) {
+#pragma unroll
+          for (int s = 0; s < 2; ++s)
+            if (!turns || s == j) {
+              issue_scores<D, F16>(base + s_col(s), qs + (turns ? 0 : s * TILE), kv_addr(kv_count + 2 * j));
+              tc::commit(s_full + s);
+            }
+          tc::commit(kv_empty + (kv_count + 2 * j) % SLOTS);
+          if (j + 1 == all) tc::commit(q_empty);
+        }
+        __syncwarp();
+      }
+      if (!ok) break;
+      const int ahead = turns ? 2 : 1;  // the side's next scores
+      for (int j = 0; j < all; ++j) {
+        const uint32_t vt = kv_count + 2 * j + 1, kt = kv_count + 2 * (j + ahead);
+        ok = kv_wait(vt) && (j + ahead >= all || kv_wait(kt));
+        if (!ok) break;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          if (turns && s != (j & 1)) continue;
+          ok = ready(p_part + s, p_phase[s]);
+          if (!ok) break;
+          if (elect_one()) issue_values<D, F16>(base + o_col(s), base + s_col(s), kv_addr(vt), 0, 6, j >= ahead);
+          __syncwarp();
+          ok = ready(p_full + s, p_phase[s]);
+          if (!ok) break;
+          p_phase[s] ^= 1;
+          if (elect_one()) {
+            issue_values<D, F16>(base + o_col(s), base + s_col(s), kv_addr(vt), 6, 8, true);
+            if (j + ahead >= all) {
+              tc::commit(o_full + s);
+            } else {
+              issue_scores<D, F16>(base + s_col(s), qs + (turns ? 0 : s * TILE), kv_addr(kt));
+              tc::commit(s_full + s);
+            }
+            if (turns || s == 1) {  // the last use of these tiles
+              tc::commit(kv_empty + vt % SLOTS);
+              if (j + ahead < all) tc::commit(kv_empty + kt % SLOTS);
+              if (j + ahead + 1 == all) tc::commit(q_empty);
+            }
+          }
+          __syncwarp();
+        }
+        if (!ok) break;
+      }
+      if (!ok) break;
+      kv_count += 2 * all;
+      if (lane == 0) tc::mbar_arrive(unit_empty + us);
+    }
+    // every product is done before the TMEM goes (at once, unless a wait gave up)
+    if (elect_one()) tc::commit(drain);
+    __syncwarp();
+    settle(drain, 0, a.status);
+  } else {
+    // ---------------------------------------------------------------- shares and page loads
+    const bool report = blockIdx.x == 0;
+    long long all = 0;
+    for (int s = lane; s < a.seqs; s += 32) all += seq_tiles(a, seq_work(a, s, report));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+    const int used = used_ctas(a, all);
+    long long at = (int)blockIdx.x < used ? share(all, used, blockIdx.x) : all;
+    const long long end = (int)blockIdx.x < used ? share(all, used, blockIdx.x + 1) : all;
+    // the sequence that holds tile `at`, and the tiles before it
+    int seq = 0;
+    long long before = 0;
+    if (at < end) {
+      for (;; seq += 32) {
+        const long long mine = seq + lane < a.seqs ? seq_tiles(a, seq_work(a, seq + lane, false)) : 0;
+        long long upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+          if (lane >= o) upto += v;
+        }
+        const uint32_t past = __ballot_sync(0xffffffffu, before + upto > at);
+        if (past) {
+          const int l = __ffs(past) - 1;
+          seq += l;
+          before += __shfl_sync(0xffffffffu, upto - mine, l);
+          break;
+        }
+        before += __shfl_sync(0xffffffffu, upto, 31);
+      }
+    }
+    SeqWork w = {0, 0, 0, 0, 0};
+    if (at < end) w = seq_work(a, seq, false);
+    uint32_t kv_count = 0, q_count = 0;
+    bool ok = true;
+    for (int k = 0; ok; ++k) {
+      Unit u = {0, 0, 0, -1, 0, 0, 0, -1, 0, 0};
+      if (at < end) {
+        while (at >= before + seq_tiles(a, w)) {
+          before += seq_tiles(a, w);
+          w = seq_work(a, ++seq, false);
+        }
+        const long long item = (at - before) / w.tiles, item0 = before + item * w.tiles;
+        u.first = w.first;
+        u.n = w.n;
+        u.node = (int)(item % w.parts) * 2 * a.nodes;
+        u.head = (int)(item / w.parts);
+        u.seq = seq;
+        u.t0 = (int)(at - item0);
+        u.t1 = (int)min((long long)w.tiles, end - item0);
+        u.ctx = w.ctx;
+        if (u.t0 > 0) u.slot = 2 * blockIdx.x;
+        else if (u.t1 < w.tiles) u.slot = 2 * blockIdx.x + 1;
+      }
+      const int us = k % kUnits;
+      ok = __all_sync(0xffffffffu, wait(unit_empty + us, ((k / kUnits) & 1) ^ 1, ending, a.status));
+      if (!ok) break;
+      if (lane == 0) {
+        units[us] = u;
+        tc::mbar_arrive(unit_full + us);
+      }
+      __syncwarp();
+      if (u.head < 0) break;
+      at += u.t1 - u.t0;
+      ok = __all_sync(0xffffffffu, wait(q_empty, (q_count & 1) ^ 1, ending, a.status));
+      if (!ok) break;
+      ++q_count;
+      const bool turns = in_turn(a, u);
+      if (lane == 0) {
+        const int sides = turns ? 1 : 2;
+        tc::mbar_arrive_expect_tx(q_full, sides * a.nodes * a.group * D * 2);
+        for (int s = 0; s < sides; ++s)
+          for (int x = 0; x < D; x += 64)
+            tma_load_3d(smem + s * TILE + x / 64 * (kRows * 128), &mq, q_full, x, u.head * a.group,
+                        u.first + u.node + s * a.nodes);
+      }
+      const int32_t* table = a.table + (long long)u.seq * a.table_pages;
+      const int held = (int)((u.ctx + u.n + kPageTokens - 1) >> kPageLog2);  // pages of the sequence
+      int pages[2] = {0, 0};
+      for (int j = 0; j < 2 * (u.t1 - u.t0); ++j, ++kv_count) {
+        const int slot = kv_count % SLOTS, tile = u.t0 + (j >> 1);
+        const int count = min(2, held - 2 * tile);
+        if (!(j & 1)) {
+          for (int h = 0; h < count; ++h) {
+            pages[h] = table[2 * tile + h];
+            if (pages[h] < 0 || pages[h] >= a.pages) {  // any page in its place: the rows are void
+              if (lane == 0) status_or(a.status, YUE2_STATUS_PAGE);
+              pages[h] = 0;
+            }
+          }
+        }
+        ok = __all_sync(0xffffffffu, wait(kv_empty + slot, ((kv_count / SLOTS) & 1) ^ 1, ending, a.status));
+        if (!ok) break;
+        if (lane == 0) {
+          tc::mbar_arrive_expect_tx(kv_full + slot, count * kPageTokens * D * 2);
+          unsigned char* dst = smem + L::OFF_KV + slot * TILE;
+          for (int h = 0; h < count; ++h) {
+            const int row = (int)(((long long)pages[h] * a.blocks + (a.layer * 2 + (j & 1)) * a.kv + u.head) * kPageTokens);
+            for (int x = 0; x < D; x += 64)
+              tc::tma_load_2d(dst + x / 64 * (kRows * 128) + h * (kPageTokens * 128), &mkv, kv_full + slot, x, row);
+          }
+        }
+        __syncwarp();
+      }
+    }
+    // no copy in flight outlives the CTA (when a wait gave up, some may not have been used)
+    if (!ok) {
+      for (uint32_t i = kv_count > SLOTS ? kv_count - SLOTS : 0; i < kv_count; ++i)
+        settle(kv_full + i % SLOTS, (i / SLOTS) & 1, a.status);
+      if (q_count) settle(q_full, (q_count - 1) & 1, a.status);
+    }
+  }
+  tc::fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc::fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+  }
+}
+
+// Rows of items that were cut: the partial results of their shares, in tile order. One CTA per row,
+// a warp per head.
+template <int D, bool F16>
+__global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(const TreeArgs a) {
+  __shared__ int s_seq;
+  __shared__ long long s_sum[2][kMergeThreads / 32];
+  const int row = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) s_seq = a.seqs;
+  __syncthreads();
+  for (int s = threadIdx.x; s < a.seqs; s += kMergeThreads) {
+    const SeqWork w = seq_work(a, s, false);
+    if (row >= w.first && row < w.first + w.n) atomicMin(&s_seq, s);
+  }
+  __syncthreads();
+  const int seq = s_seq;
+  long long sums[2] = {0, 0};  // tiles of all sequences, and of those before this one
+  for (int s = threadIdx.x; s < a.seqs; s += kMergeThreads) {
+    const long long n = seq_tiles(a, seq_work(a, s, false));
+    sums[0] += n;
+    if (s < seq) sums[1] += n;
+  }
+  for (int i = 0; i < 2; ++i) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sums[i] += __shfl_xor_sync(0xffffffffu, sums[i], o);
+    if (lane == 0) s_sum[i][warp] = sums[i];
+  }
+  __syncthreads();
+  long long all = 0, before = 0;
+  for (int i = 0; i < kMergeThreads / 32; ++i) all += s_sum[0][i], before += s_sum[1][i];
+  pdl_wait();  // by every thread, whatever its row
+  if (seq == a.seqs) return;
+  const SeqWork w = seq_work(a, seq, false);
+  const int used = used_ctas(a, all);
+  const int node = row - w.first, block = node / (2 * a.nodes);
+  constexpr int E = D / 32;
+  const float2* stats = reinterpret_cast<const float2*>(a.part + 2ll * a.ctas * a.slot_rows * D);
+  for (int h = warp; h < a.heads; h += kMergeThreads / 32) {
+    const long long x0 = before + ((long long)(h / a.group) * w.parts + block) * w.tiles;
+    const int c0 = owner(all, used, x0), c1 = owner(all, used, x0 + w.tiles - 1);
+    if (c0 == c1) continue;  // finished by its CTA
+    const long long r = (node - block * 2 * a.nodes) * a.group + h % a.group;
+    float m = -INFINITY;
+    for (int c = c0; c <= c1; ++c) m = max3(m, stats[(2ll * c + (c == c0)) * a.slot_rows + r].x, -INFINITY);
+    float l = 0.f, o[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = 0.f;
+    for (int c = c0; c <= c1; ++c) {
+      const long long at = (2ll * c + (c == c0)) * a.slot_rows + r;
+      const float2 s = stats[at];
+      if (s.x == -INFINITY) continue;  // no key seen in this share
+      // not below the smallest normal number, so that infinities stay what they are
+      const float f = max3(ex2((s.x - m) * a.c), 1.17549435e-38f, 0.f);
+      l = fmaf(s.y, f, l);
+      const float* p = a.part + at * D + lane * E;
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] = fmaf(p[e], f, o[e]);
+    }
+    const float inv = l > 0.f ? 1.0f / l : l == 0.f ? 0.f : l;
+    uint16_t* dst = a.out + (long long)row * a.out_stride + (long long)h * D + lane * E;
+#pragma unroll
+    for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = pack16<F16>(o[e] * inv, o[e + 1] * inv);
+  }
+}
+
+int sm_count(int& sms) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  return e == cudaSuccess ? 0 : cuda_fail(e, "device attributes");
+}
+
+// Nodes of a side, CTAs and the rows of a partial result.
+struct Plan {
+  int nodes, ctas, slot_rows;
+  uint64_t bytes;
+};
+Plan plan_for(uint64_t rows, uint64_t heads, uint64_t kv, uint64_t dim, uint64_t seqs, uint64_t table_pages, int sms) {
+  Plan p;
+  const uint64_t group = heads / kv;
+  p.nodes = (int)(kRows / group);
+  const uint64_t most = std::min<uint64_t>(rows, kMaxNodes);  // of one sequence
+  const uint64_t parts = (most + 2 * p.nodes - 1) / (2 * p.nodes), tiles = (table_pages + 1) / 2;
+  p.ctas = (int)std::max<uint64_t>(1, std::min<uint64_t>(sms, std::min<uint64_t>(seqs, rows) * kv * parts * tiles));
+  p.slot_rows = (int)(std::min<uint64_t>(most, 2 * p.nodes) * group);
+  p.bytes = tiles > 1 ? 2ull * p.ctas * p.slot_rows * (dim + 2) * 4 : 0;
+  return p;
+}
+
+template <int D, bool F16>
+int launch(const CUtensorMap& mq, const CUtensorMap& mkv, const TreeArgs& a, bool merge, cudaStream_t st) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
+  static std::atomic<uint64_t> ready{0};  // devices on which the shared-memory limit is set
+  if (dev >= 64 || !(ready.load(std::memory_order_relaxed) >> dev & 1)) {
+    e = cudaFuncSetAttribute(attention_tree_kernel<D, F16>, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<D>::BYTES);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute");
+    if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
+  }
+  attention_tree_kernel<D, F16><<<(unsigned)a.ctas, kThreads, Layout<D>::BYTES, st>>>(mq, mkv, a);
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return cuda_fail(e, "attention_tree launch");
+  if (!merge) return 0;
+  TreeArgs copy = a;
+  void* args[] = {&copy};
+  e = launch_with(st, true, dim3((unsigned)a.rows), dim3(kMergeThreads), 0, (const void*)tree_merge_kernel<D, F16>, args);
+  return e == cudaSuccess ? 0 : cuda_fail(e, "attention_tree merge launch");
 }
 
 }  // namespace
@@ -115,16 +640,23 @@ using namespace y2;
 
 extern "C" {
 
-uint64_t yue2_attention_tree_workspace(uint64_t, uint64_t, uint64_t, uint64_t, const Yue2KvPool*) { return 0; }
+uint64_t yue2_attention_tree_workspace(uint64_t rows, uint64_t heads, uint64_t seqs, uint64_t table_pages,
+                                       const Yue2KvPool* pool) {
+  int sms = 0;
+  if (!pool || !rows || !seqs || !heads || !pool->kv || heads % pool->kv || heads / pool->kv > kMaxGroup || sm_count(sms))
+    return 0;
+  return plan_for(rows, heads, pool->kv, pool->dim, seqs, table_pages, sms).bytes;
+}
 
 int yue2_attention_tree(const void* q, uint64_t rows, uint64_t heads, uint64_t q_stride, const Yue2KvPool* pool,
                         uint64_t layer, const int32_t* table, uint64_t seqs, uint64_t table_pages,
                         const int32_t* context, const int32_t* cu, const uint64_t* mask, float scale, void* out,
                         uint64_t out_stride, void* workspace, uint64_t workspace_bytes, int32_t* status,
                         void* stream) {
-  TreeParams p = {};
-  int rc = check_pool(pool, true, p.pool);
+  PoolView v = {};
+  int rc = check_pool(pool, true, v);
   if (rc || (rc = check_heads(heads, pool->kv)) || (rc = check_status(status)) || (rc = check_scale(scale))) return rc;
+  if (heads / pool->kv > kMaxGroup) return fail(YUE2_ERR_INVALID, "at most 128 query heads per kv head");
   if (layer >= pool->layers) return fail(YUE2_ERR_INVALID, "layer outside the KV pool");
   if (seqs > (uint64_t)kMaxSeqs || table_pages > (1u << 24))
     return fail(YUE2_ERR_INVALID, "at most 1,024 sequences and 2^24 pages per table row");
@@ -134,35 +666,50 @@ int yue2_attention_tree(const void* q, uint64_t rows, uint64_t heads, uint64_t q
     return rc;
   if (seqs == 0 || rows == 0) return 0;
   if (!table || !context || !cu) return fail(YUE2_ERR_INVALID, "null page table, context or row offsets");
-  (void)workspace;
-  (void)workspace_bytes;
-  p.q = (const uint16_t*)q;
-  p.out = (uint16_t*)out;
-  p.table = table;
-  p.context = context;
-  p.cu = cu;
-  p.mask = mask;
-  p.status = status;
-  p.q_stride = (long long)q_stride;
-  p.out_stride = (long long)out_stride;
-  p.table_pages = (long long)table_pages;
-  p.seqs = (int)seqs;
-  p.rows = (int)rows;
-  p.heads = (int)heads;
-  p.layer = (int)layer;
-  p.scale = scale;
-  const dim3 grid((unsigned)rows);
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const uint64_t pool_rows = (uint64_t)v.pages * v.blocks * kPageTokens;
+  if (pool_rows > (uint64_t)INT32_MAX) return fail(YUE2_ERR_INVALID, "the KV pool has more than 2^31 head rows");
+  int sms = 0;
+  if ((rc = sm_count(sms))) return rc;
+  const Plan plan = plan_for(rows, heads, pool->kv, pool->dim, seqs, table_pages, sms);
+  if (plan.bytes && (!workspace || !aligned16(workspace) || workspace_bytes < plan.bytes))
+    return fail(YUE2_ERR_INVALID, "the workspace must be 16-byte aligned and hold yue2_attention_tree_workspace bytes");
   const bool f16 = pool->dtype == YUE2_DTYPE_F16;
-  if (p.pool.dim == 64) {
-    if (f16) tree_kernel<64, true><<<grid, 128, 0, st>>>(p);
-    else tree_kernel<64, false><<<grid, 128, 0, st>>>(p);
-  } else {
-    if (f16) tree_kernel<128, true><<<grid, 128, 0, st>>>(p);
-    else tree_kernel<128, false><<<grid, 128, 0, st>>>(p);
-  }
-  const cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? 0 : cuda_fail(e, "attention_tree launch");
+  const uint64_t dim = pool->dim;
+  CUtensorMap mq, mkv;
+  const cuuint64_t dims[2] = {dim, pool_rows}, strides[1] = {dim * 2};
+  if (!opt::make_rows_map(&mq, f16, q, rows, heads, dim, q_stride, (int)(heads / pool->kv), plan.nodes) ||
+      !opt::make_map(&mkv, f16, pool->base, 2, dims, strides, kPageTokens, 1))
+    return fail(YUE2_ERR_INVALID, "q or the KV pool cannot be described to the copy engine (base, strides)");
+  TreeArgs a = {};
+  a.out = (uint16_t*)out;
+  a.pool = v.base;
+  a.table = table;
+  a.context = context;
+  a.cu = cu;
+  a.mask = mask;
+  a.status = status;
+  a.part = (float*)workspace;
+  a.out_stride = (long long)out_stride;
+  a.pages = v.pages;
+  a.page_stride = v.page_stride;
+  a.table_pages = (long long)table_pages;
+  a.seqs = (int)seqs;
+  a.rows = (int)rows;
+  a.heads = (int)heads;
+  a.kv = v.kv;
+  a.group = (int)(heads / pool->kv);
+  a.nodes = plan.nodes;
+  a.layer = (int)layer;
+  a.blocks = v.blocks;
+  a.negate = scale < 0.f;
+  a.ctas = plan.ctas;
+  a.slot_rows = plan.slot_rows;
+  // not below the smallest normal number: a masked score is -inf, and 0 * -inf is not 0
+  a.c = std::max(std::fabs(scale) * 1.4426950408889634f, 1.17549435e-38f);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool merge = plan.bytes > 0;
+  if (dim == 64) return f16 ? launch<64, true>(mq, mkv, a, merge, st) : launch<64, false>(mq, mkv, a, merge, st);
+  return f16 ? launch<128, true>(mq, mkv, a, merge, st) : launch<128, false>(mq, mkv, a, merge, st);
 }
 
 }  // extern "C"

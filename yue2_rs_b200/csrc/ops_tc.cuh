@@ -6,7 +6,9 @@
 // probabilities go back over S as packed 16-bit pairs and are the A operand of O += P.V from
 // TMEM, V being the [keys][dim] tile as it lies in memory (the MN-major B operand).
 #pragma once
-#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <atomic>
 
 #include "ops.cuh"
 #include "tcgen05.cuh"
@@ -269,7 +271,8 @@ Y2_DEV void softmax_tile(uint32_t s_addr, uint32_t o_addr, float c, bool negate,
   }
   load32(s_addr, v[0]);
   const float mn = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]);
-  const bool move = first || !((mn - st.m) * c <= 8.0f);  // NaN moves too
+  // NaN moves too; a row that has seen nothing yet stays
+  const bool move = first || (mn != -INFINITY && !((mn - st.m) * c <= 8.0f));
   if (!first && __any_sync(0xffffffffu, move)) {
     const float alpha = move ? ex2((st.m - mn) * c) : 1.0f;
 #pragma unroll
@@ -353,6 +356,34 @@ Y2_DEV void add_nonfinite(const uint16_t* v, float (&o)[32]) {
     for (int e = 0; e < 8; ++e)
       if (!isfinite(x[e])) o[i + e] += x[e];
   }
+}
+
+// ---- host
+// Tensor map of 16-bit values [.., dims[1], dims[0]] (strides in bytes of the outer
+// dimensions) in boxes of 64 x box1 x box2 values, 128-byte swizzle, zeros beyond the end. The
+// driver's encoder is looked up through the runtime, so that the library loads without a driver.
+inline bool make_map(CUtensorMap* m, bool f16, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides,
+                     cuuint32_t box1, cuuint32_t box2) {
+  static std::atomic<void*> found{nullptr};
+  void* fn = found.load(std::memory_order_relaxed);
+  if (!fn) {
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      return false;
+    found.store(fn, std::memory_order_relaxed);
+  }
+  const cuuint32_t box[3] = {64, box1, box2}, step[3] = {1, 1, 1};
+  return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn)(
+             m, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (cuuint32_t)rank,
+             const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+// [rows, heads, dim] values with a row stride in elements, in boxes of [box_rows][box_heads][64].
+inline bool make_rows_map(CUtensorMap* m, bool f16, const void* base, uint64_t rows, uint64_t heads, uint64_t dim,
+                          uint64_t stride, int box_heads, int box_rows) {
+  const cuuint64_t dims[3] = {dim, heads, rows}, strides[2] = {dim * 2, stride * 2};
+  return make_map(m, f16, base, 3, dims, strides, (cuuint32_t)box_heads, (cuuint32_t)box_rows);
 }
 
 }  // namespace opt
