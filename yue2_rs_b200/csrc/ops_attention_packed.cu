@@ -242,7 +242,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc::fence_after();
         const float inv = 1.0f / st.total();
         const bool found = *(volatile int*)&units[us].found;
-        uint16_t* dst = a.out + (long long)(u.first + row) * a.out_stride + u.head * D;
+        char* to[4];
+        quad_rows(t < rows ? a.out + (long long)(u.first + row) * a.out_stride + u.head * D : nullptr, to);
 #pragma unroll 1
         for (int q = 0; q < D / 32; ++q) {
           uint32_t o[32];
@@ -255,15 +256,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (found && t < rows)  // keys of the unit's masked tiles that this row sees
             for (int key = u.block * kBlock; key <= last; ++key)
               add_nonfinite<F16>(a.v + (long long)(u.first + key) * a.v_stride + (u.head / a.group) * D + 32 * q, f);
-          if (t < rows) {
-#pragma unroll
-            for (int i = 0; i < 32; i += 8) {
-              float x[8];
-#pragma unroll
-              for (int e = 0; e < 8; ++e) x[e] = f[i + e];
-              *reinterpret_cast<uint4*>(dst + 32 * q + i) = pack8<F16>(x);
-            }
-          }
+          uint4 w[4];
+          pack32<F16>(f, w);
+          quad_store(to, 64 * q, w);
         }
         tc::fence_before();
       }

@@ -7,8 +7,8 @@
 // rows fill one side, both sides hold them and take the tiles in turn, and their results are
 // merged in TMEM: two softmax warps then keep up with HBM even when a single warp has rows.
 //
-// The tiles of all items form one line, cut into equal shares for the CTAs (one per SM), so
-// that one long context among short ones loads every SM alike. An item cut between CTAs
+// The items form one line (a fixed cost, then their tiles), cut into equal shares for the CTAs
+// (one per SM), so that one long context among short ones loads every SM alike. An item cut between CTAs
 // leaves partial results (output, maximum and sum, f32) that a second kernel merges in tile
 // order; items that lie in one share are finished at once. The shares follow from the
 // lengths on the device, so the host needs none of them.
@@ -66,18 +66,28 @@ Y2_DEV SeqWork seq_work(const TreeArgs& a, int s, bool report) {
   w.parts = (w.n + 2 * a.nodes - 1) / (2 * a.nodes);
   return w;
 }
-Y2_DEV long long seq_tiles(const TreeArgs& a, const SeqWork& w) { return (long long)w.tiles * w.parts * a.kv; }
 
-// Shares: CTA c of `used` takes tiles [share(c), share(c + 1)) of `all`.
-Y2_DEV int used_ctas(const TreeArgs& a, long long all) { return (int)min((long long)a.ctas, max(all, 1ll)); }
-Y2_DEV long long share(long long all, int used, int c) { return all * c / used; }
-// The CTA whose share holds tile x.
-Y2_DEV int owner(long long all, int used, long long x) {
-  int c = (int)(x * used / all);
-  while (share(all, used, c) > x) --c;
-  while (share(all, used, c + 1) <= x) ++c;
-  return c;
+// The line of work: an item is kItemCost units (its loads of q, masked tiles and output
+// take about as long as that many tiles) and then one unit a tile. CTA c of `used` takes the
+// units [share(c), share(c + 1)). Lines of 2^31 units and more are refused.
+constexpr int kItemCost = 2;
+Y2_DEV int item_length(const SeqWork& w) { return w.n ? w.tiles + kItemCost : 0; }
+Y2_DEV int seq_length(const TreeArgs& a, const SeqWork& w) {
+  return (int)min((long long)INT32_MAX, (long long)item_length(w) * w.parts * a.kv);
 }
+struct Shares {
+  int used, each, more;  // the first `more` CTAs take one unit more than `each`
+  Y2_DEV Shares(const TreeArgs& a, int all) {
+    used = min(a.ctas, max(all, 1));
+    each = all / used;
+    more = all % used;
+  }
+  Y2_DEV int begin(int c) const { return c * each + min(c, more); }
+  Y2_DEV int owner(int x) const {
+    const int wide = more * (each + 1);
+    return x < wide ? x / (each + 1) : more + (x - wide) / each;
+  }
+};
 
 struct Unit {
   int first, n, node, head;  // the sequence's rows, the block's first node, the kv head (< 0: end)
@@ -268,8 +278,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool found = *(volatile int*)&units[us].found;
         const float inv = l > 0.f ? 1.0f / l : l == 0.f ? 0.f : l;  // nothing seen: zeros
         const int row = u.first + node, head = u.head * a.group + t % a.group;
-        uint16_t* dst = a.out + (long long)row * a.out_stride + (long long)head * D;
         const long long prow = (long long)u.slot * a.slot_rows + (node - u.node) * a.group + t % a.group;
+        void* mine = u.slot >= 0 ? (void*)(a.part + prow * D) : (void*)(a.out + (long long)row * a.out_stride + (long long)head * D);
+        char* to[4];
+        quad_rows(live ? mine : nullptr, to);
 #pragma unroll 1
         for (int q = 0; q < D / 32; ++q) {
           uint32_t o[32];
@@ -300,19 +312,22 @@ __global__ void __launch_bounds__(kThreads, 1)
                                  f);
             }
           }
-          if (!live) continue;
+          uint4 v[4];
           if (u.slot >= 0) {
-            float4* p = reinterpret_cast<float4*>(a.part + prow * D + 32 * q);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) p[i] = make_float4(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]);
+            for (int h = 0; h < 2; ++h) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float* x = f + 16 * h + 4 * i;
+                v[i] = make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+              }
+              quad_store(to, 128 * q + 64 * h, v);
+            }
           } else {
 #pragma unroll
-            for (int i = 0; i < 32; i += 8) {
-              float x[8];
-#pragma unroll
-              for (int e = 0; e < 8; ++e) x[e] = f[i + e] * inv;
-              *reinterpret_cast<uint4*>(dst + 32 * q + i) = pack8<F16>(x);
-            }
+            for (int i = 0; i < 32; ++i) f[i] *= inv;
+            pack32<F16>(f, v);
+            quad_store(to, 64 * q, v);
           }
         }
         if (live && u.slot >= 0)
@@ -406,30 +421,33 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else {
     // ---------------------------------------------------------------- shares and page loads
     const bool report = blockIdx.x == 0;
-    long long all = 0;
-    for (int s = lane; s < a.seqs; s += 32) all += seq_tiles(a, seq_work(a, s, report));
+    long long sum = 0;
+    for (int s = lane; s < a.seqs; s += 32) sum += seq_length(a, seq_work(a, s, report));
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
-    const int used = used_ctas(a, all);
-    long long at = (int)blockIdx.x < used ? share(all, used, blockIdx.x) : all;
-    const long long end = (int)blockIdx.x < used ? share(all, used, blockIdx.x + 1) : all;
-    // the sequence that holds tile `at`, and the tiles before it
-    int seq = 0;
-    long long before = 0;
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    const bool fits = sum < INT32_MAX;
+    if (!fits && report && lane == 0) status_or(a.status, YUE2_STATUS_RANGE);
+    const int all = fits ? (int)sum : 0;
+    const Shares shares(a, all);
+    const bool mine = (int)blockIdx.x < shares.used;
+    int at = mine ? shares.begin(blockIdx.x) : all;
+    const int end = mine ? shares.begin(blockIdx.x + 1) : all;
+    // the sequence that holds unit `at`, and the units before it
+    int seq = 0, before = 0;
     if (at < end) {
       for (;; seq += 32) {
-        const long long mine = seq + lane < a.seqs ? seq_tiles(a, seq_work(a, seq + lane, false)) : 0;
-        long long upto = mine;
+        const int own = seq + lane < a.seqs ? seq_length(a, seq_work(a, seq + lane, false)) : 0;
+        int upto = own;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-          const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+          const int v = __shfl_up_sync(0xffffffffu, upto, o);
           if (lane >= o) upto += v;
         }
         const uint32_t past = __ballot_sync(0xffffffffu, before + upto > at);
         if (past) {
           const int l = __ffs(past) - 1;
           seq += l;
-          before += __shfl_sync(0xffffffffu, upto - mine, l);
+          before += __shfl_sync(0xffffffffu, upto - own, l);
           break;
         }
         before += __shfl_sync(0xffffffffu, upto, 31);
@@ -437,26 +455,31 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     SeqWork w = {0, 0, 0, 0, 0};
     if (at < end) w = seq_work(a, seq, false);
+    int length = item_length(w), total = seq_length(a, w);
     uint32_t kv_count = 0, q_count = 0;
     bool ok = true;
     for (int k = 0; ok; ++k) {
       Unit u = {0, 0, 0, -1, 0, 0, 0, -1, 0, 0};
-      if (at < end) {
-        while (at >= before + seq_tiles(a, w)) {
-          before += seq_tiles(a, w);
+      while (at < end) {
+        while (at >= before + total) {
+          before += total;
           w = seq_work(a, ++seq, false);
+          length = item_length(w), total = seq_length(a, w);
         }
-        const long long item = (at - before) / w.tiles, item0 = before + item * w.tiles;
+        const int item = (at - before) / length, item0 = before + item * length;
+        u.t0 = max(0, at - item0 - kItemCost);
+        u.t1 = min(w.tiles, end - item0 - kItemCost);
+        at = min(end, item0 + length);
+        if (u.t1 <= u.t0) continue;  // only of the fixed cost: the next CTA has the tiles
         u.first = w.first;
         u.n = w.n;
-        u.node = (int)(item % w.parts) * 2 * a.nodes;
-        u.head = (int)(item / w.parts);
+        u.node = (item % w.parts) * 2 * a.nodes;
+        u.head = item / w.parts;
         u.seq = seq;
-        u.t0 = (int)(at - item0);
-        u.t1 = (int)min((long long)w.tiles, end - item0);
         u.ctx = w.ctx;
         if (u.t0 > 0) u.slot = 2 * blockIdx.x;
         else if (u.t1 < w.tiles) u.slot = 2 * blockIdx.x + 1;
+        break;
       }
       const int us = k % kUnits;
       ok = __all_sync(0xffffffffu, wait(unit_empty + us, ((k / kUnits) & 1) ^ 1, ending, a.status));
@@ -467,7 +490,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       __syncwarp();
       if (u.head < 0) break;
-      at += u.t1 - u.t0;
       ok = __all_sync(0xffffffffu, wait(q_empty, (q_count & 1) ^ 1, ending, a.status));
       if (!ok) break;
       ++q_count;
@@ -524,27 +546,25 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// Rows of items that were cut: the partial results of their shares, in tile order. One CTA per row,
-// a warp per head.
+// Rows of items that were cut: the partial results of their shares, in tile order. A CTA takes
+// eight heads of a row, a warp each.
 template <int D, bool F16>
 __global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(const TreeArgs a) {
   __shared__ int s_seq;
   __shared__ long long s_sum[2][kMergeThreads / 32];
   const int row = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int h = blockIdx.y * (kMergeThreads / 32) + warp;
   if (threadIdx.x == 0) s_seq = a.seqs;
   __syncthreads();
+  long long sums[2] = {0, 0};  // units of all sequences, and of those before this one
   for (int s = threadIdx.x; s < a.seqs; s += kMergeThreads) {
     const SeqWork w = seq_work(a, s, false);
     if (row >= w.first && row < w.first + w.n) atomicMin(&s_seq, s);
+    sums[0] += seq_length(a, w);
   }
   __syncthreads();
   const int seq = s_seq;
-  long long sums[2] = {0, 0};  // tiles of all sequences, and of those before this one
-  for (int s = threadIdx.x; s < a.seqs; s += kMergeThreads) {
-    const long long n = seq_tiles(a, seq_work(a, s, false));
-    sums[0] += n;
-    if (s < seq) sums[1] += n;
-  }
+  for (int s = threadIdx.x; s < seq; s += kMergeThreads) sums[1] += seq_length(a, seq_work(a, s, false));
   for (int i = 0; i < 2; ++i) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sums[i] += __shfl_xor_sync(0xffffffffu, sums[i], o);
@@ -554,38 +574,52 @@ __global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(const TreeArg
   long long all = 0, before = 0;
   for (int i = 0; i < kMergeThreads / 32; ++i) all += s_sum[0][i], before += s_sum[1][i];
   pdl_wait();  // by every thread, whatever its row
-  if (seq == a.seqs) return;
+  if (seq == a.seqs || h >= a.heads || all >= INT32_MAX) return;
   const SeqWork w = seq_work(a, seq, false);
-  const int used = used_ctas(a, all);
-  const int node = row - w.first, block = node / (2 * a.nodes);
+  const Shares shares(a, (int)all);
+  const int node = row - w.first, block = node / (2 * a.nodes), length = item_length(w);
+  const int x0 = (int)before + ((h / a.group) * w.parts + block) * length;
+  const int c0 = shares.owner(x0 + kItemCost), c1 = shares.owner(x0 + length - 1);
+  if (c0 == c1) return;  // finished by its CTA
   constexpr int E = D / 32;
   const float2* stats = reinterpret_cast<const float2*>(a.part + 2ll * a.ctas * a.slot_rows * D);
-  for (int h = warp; h < a.heads; h += kMergeThreads / 32) {
-    const long long x0 = before + ((long long)(h / a.group) * w.parts + block) * w.tiles;
-    const int c0 = owner(all, used, x0), c1 = owner(all, used, x0 + w.tiles - 1);
-    if (c0 == c1) continue;  // finished by its CTA
-    const long long r = (node - block * 2 * a.nodes) * a.group + h % a.group;
-    float m = -INFINITY;
-    for (int c = c0; c <= c1; ++c) m = max3(m, stats[(2ll * c + (c == c0)) * a.slot_rows + r].x, -INFINITY);
-    float l = 0.f, o[E];
+  const long long r = (node - block * 2 * a.nodes) * a.group + h % a.group;
+  auto slot = [&](int c) { return (2ll * c + (c == c0)) * a.slot_rows + r; };
+  float m = -INFINITY;
+  for (int c = c0 + lane; c <= c1; c += 32) m = max3(m, stats[slot(c)].x, -INFINITY);
 #pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = 0.f;
-    for (int c = c0; c <= c1; ++c) {
-      const long long at = (2ll * c + (c == c0)) * a.slot_rows + r;
-      const float2 s = stats[at];
-      if (s.x == -INFINITY) continue;  // no key seen in this share
-      // not below the smallest normal number, so that infinities stay what they are
-      const float f = max3(ex2((s.x - m) * a.c), 1.17549435e-38f, 0.f);
+  for (int o = 16; o > 0; o >>= 1) m = max3(m, __shfl_xor_sync(0xffffffffu, m, o), -INFINITY);
+  float l = 0.f, o[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) o[e] = 0.f;
+  for (int base = c0; base <= c1; base += 32) {
+    float f = 0.f;
+    if (base + lane <= c1) {
+      const float2 s = stats[slot(base + lane)];
+      // not below the smallest normal number, so that infinities stay what they are; a share in
+      // which the row saw nothing has none
+      f = s.x == -INFINITY ? 0.f : max3(ex2((s.x - m) * a.c), 1.17549435e-38f, 0.f);
       l = fmaf(s.y, f, l);
-      const float* p = a.part + at * D + lane * E;
-#pragma unroll
-      for (int e = 0; e < E; ++e) o[e] = fmaf(p[e], f, o[e]);
     }
-    const float inv = l > 0.f ? 1.0f / l : l == 0.f ? 0.f : l;
-    uint16_t* dst = a.out + (long long)row * a.out_stride + (long long)h * D + lane * E;
-#pragma unroll
-    for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = pack16<F16>(o[e] * inv, o[e + 1] * inv);
+    const int n = min(32, c1 - base + 1);
+#pragma unroll 4
+    for (int i = 0; i < n; ++i) {
+      const float fi = __shfl_sync(0xffffffffu, f, i);
+      const float* p = a.part + slot(base + i) * D + lane * E;
+      if constexpr (E == 4) {
+        const float4 x = *reinterpret_cast<const float4*>(p);
+        o[0] = fmaf(x.x, fi, o[0]), o[1] = fmaf(x.y, fi, o[1]), o[2] = fmaf(x.z, fi, o[2]), o[3] = fmaf(x.w, fi, o[3]);
+      } else {
+        const float2 x = *reinterpret_cast<const float2*>(p);
+        o[0] = fmaf(x.x, fi, o[0]), o[1] = fmaf(x.y, fi, o[1]);
+      }
+    }
   }
+  l = warp_sum(l);
+  const float inv = l > 0.f ? 1.0f / l : l == 0.f ? 0.f : l;
+  uint16_t* dst = a.out + (long long)row * a.out_stride + (long long)h * D + lane * E;
+#pragma unroll
+  for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = pack16<F16>(o[e] * inv, o[e + 1] * inv);
 }
 
 int sm_count(int& sms) {
@@ -629,7 +663,7 @@ int launch(const CUtensorMap& mq, const CUtensorMap& mkv, const TreeArgs& a, boo
   if (!merge) return 0;
   TreeArgs copy = a;
   void* args[] = {&copy};
-  e = launch_with(st, true, dim3((unsigned)a.rows), dim3(kMergeThreads), 0, (const void*)tree_merge_kernel<D, F16>, args);
+  e = launch_with(st, true, dim3((unsigned)a.rows, (unsigned)((a.heads + 7) / 8)), dim3(kMergeThreads), 0, (const void*)tree_merge_kernel<D, F16>, args);
   return e == cudaSuccess ? 0 : cuda_fail(e, "attention_tree merge launch");
 }
 

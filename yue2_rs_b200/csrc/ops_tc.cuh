@@ -226,8 +226,15 @@ Y2_DEV void poly_ex2(float& x, float& y) {
 template <bool PLAIN>
 Y2_DEV void take_scores(uint32_t (&v)[32], bool negate, uint32_t vis) {
   if constexpr (!PLAIN) {
+    if (negate) {
 #pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = vis >> i & 1 ? v[i] ^ (negate ? 0x80000000u : 0u) : 0xff800000u;
+      for (int i = 0; i < 32; ++i) v[i] ^= 0x80000000u;
+    }
+    if (!__all_sync(0xffffffffu, vis == 0xffffffffu)) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (!(vis >> i & 1)) v[i] = 0xff800000u;
+    }
   }
 }
 
@@ -294,8 +301,15 @@ Y2_DEV void softmax_tile(uint32_t s_addr, uint32_t o_addr, float c, bool negate,
     wait_loads();
     arrived(s);
     if (q < 3) load32(s_addr + 32 * (q + 1), v[(q + 1) & 1]);
-    take_scores<PLAIN>(s, negate, vis[q]);
     uint32_t p[16];
+    if (!PLAIN && __all_sync(0xffffffffu, vis[q] == 0)) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) p[i] = 0;
+      store16(s_addr + 16 * q, p);
+      if (q == 2) part();
+      continue;
+    }
+    take_scores<PLAIN>(s, negate, vis[q]);
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       float a, b;
@@ -321,28 +335,76 @@ Y2_DEV void softmax_tile(uint32_t s_addr, uint32_t o_addr, float c, bool negate,
 // key, all of it becomes zero.
 template <bool F16>
 Y2_DEV void clean_values(unsigned char* vs, int r, bool dead, int* found) {
-  constexpr uint32_t EXP = F16 ? 0x7c00u : 0x7f80u;
+  if (dead) {
+#pragma unroll
+    for (int ch = 0; ch < 8; ++ch) *reinterpret_cast<uint4*>(vs + tc::sw128(r, ch)) = make_uint4(0, 0, 0, 0);
+    return;
+  }
+  // x * 0 summed up is NaN when some x is not finite
+  uint32_t acc[4] = {0, 0, 0, 0};
 #pragma unroll
   for (int ch = 0; ch < 8; ++ch) {
-    uint4* at = reinterpret_cast<uint4*>(vs + tc::sw128(r, ch));
-    if (dead) {
-      *at = make_uint4(0, 0, 0, 0);
-      continue;
-    }
-    uint4 w = *at;
-    uint32_t* x = reinterpret_cast<uint32_t*>(&w);
-    bool bad = false;
+    const uint4 w = *reinterpret_cast<const uint4*>(vs + tc::sw128(r, ch));
+    const uint32_t x[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      if ((x[i] & EXP) == EXP) x[i] &= 0xffff0000u, bad = true;
-      if ((x[i] >> 16 & EXP) == EXP) x[i] &= 0x0000ffffu, bad = true;
-    }
-    if (bad) {
-      *(volatile int*)found = 1;
-      __threadfence_block();
-      *at = w;
+      if constexpr (F16) asm("fma.rn.f16x2 %0, %1, %2, %0;" : "+r"(acc[i]) : "r"(x[i]), "r"(0));
+      else asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(acc[i]) : "r"(x[i]), "r"(0));
     }
   }
+  constexpr uint32_t EXP = F16 ? 0x7c00u : 0x7f80u;
+  auto bad = [](uint32_t w) { return (w & EXP) == EXP || (w >> 16 & EXP) == EXP; };
+  if (!(bad(acc[0]) || bad(acc[1]) || bad(acc[2]) || bad(acc[3]))) return;
+  *(volatile int*)found = 1;
+  __threadfence_block();
+#pragma unroll 1
+  for (int ch = 0; ch < 8; ++ch) {
+    uint4 w = *reinterpret_cast<uint4*>(vs + tc::sw128(r, ch));
+    uint32_t* x = reinterpret_cast<uint32_t*>(&w);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if ((x[i] & EXP) == EXP) x[i] &= 0xffff0000u;
+      if ((x[i] >> 16 & EXP) == EXP) x[i] &= 0x0000ffffu;
+    }
+    *reinterpret_cast<uint4*>(vs + tc::sw128(r, ch)) = w;
+  }
+}
+
+// Four lanes' rows, 64 bytes of each, stored 64 bytes at a time: lane i of the four ends up with
+// the i-th 16 bytes of all four rows. (A row a lane, every store would touch 32 lines; the
+// output of 256 rows took 7,000 cycles that way.) to[r]: row r of the four, null for none.
+Y2_DEV void quad_rows(void* mine, char* (&to)[4]) {
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+    to[r] = reinterpret_cast<char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine), r, 4));
+}
+Y2_DEV void quad_store(char* const (&to)[4], int offset, uint4 (&v)[4]) {
+  const int lane = threadIdx.x & 3;
+#pragma unroll
+  for (int d = 1; d < 4; d <<= 1)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (i & d) continue;
+      const bool up = lane & d;
+      uint4 s = up ? v[i] : v[i ^ d];
+      s.x = __shfl_xor_sync(0xffffffffu, s.x, d);
+      s.y = __shfl_xor_sync(0xffffffffu, s.y, d);
+      s.z = __shfl_xor_sync(0xffffffffu, s.z, d);
+      s.w = __shfl_xor_sync(0xffffffffu, s.w, d);
+      if (up) v[i] = s;
+      else v[i ^ d] = s;
+    }
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+    if (to[r]) *reinterpret_cast<uint4*>(to[r] + offset + lane * 16) = v[r];
+}
+// 32 f32 as 16-bit values, 64 bytes.
+template <bool F16>
+Y2_DEV void pack32(const float (&f)[32], uint4 (&v)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    v[i] = make_uint4(pack16<F16>(f[8 * i], f[8 * i + 1]), pack16<F16>(f[8 * i + 2], f[8 * i + 3]),
+                      pack16<F16>(f[8 * i + 4], f[8 * i + 5]), pack16<F16>(f[8 * i + 6], f[8 * i + 7]));
 }
 
 // Adds the values of a key that are not finite (32 of them at `v`) to a row's outputs.

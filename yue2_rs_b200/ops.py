@@ -14,7 +14,6 @@ the pages, `kv_gather` keeps the accepted ones, and `kv_copy` forks the last pag
 that several takes share.
 """
 import ctypes
-import math
 import threading
 
 import torch
@@ -27,7 +26,7 @@ _DTYPES = {torch.bfloat16: 0, torch.float16: 2}
 _BITS = ((1, "a page index or slot outside the pool"), (2, "a length, offset or position out of range"),
          (4, "a bounded device wait gave up"))
 
-_status = {}  # device index -> int32 status word
+_status = {}  # device index -> (address, int32 status word)
 _lock = threading.Lock()
 
 
@@ -35,18 +34,20 @@ def _invalid(message):
     return _lib.Yue2Error(-1, message)
 
 
-def _status_of(device):
-    s = _status.get(device.index)
+def _status_of(index):
+    """The address of the device's status word."""
+    s = _status.get(index)
     if s is None:
+        device = torch.device("cuda", index)
         with _lock, torch.cuda.device(device):
             if torch.cuda.is_current_stream_capturing():
                 raise _invalid("call an operator (or check_status) once on this device before any capture")
-            s = _status.get(device.index)
+            s = _status.get(index)
             if s is None:
-                s = torch.zeros(1, dtype=torch.int32, device=device)
+                word = torch.zeros(1, dtype=torch.int32, device=device)
                 torch.cuda.synchronize(device)  # cleared before any stream's kernels see it
-                _status[device.index] = s
-    return s
+                s = _status[index] = (word.data_ptr(), word)
+    return s[0]
 
 
 def check_status(device=None):
@@ -55,7 +56,8 @@ def check_status(device=None):
     device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     if device.index is None:
         device = torch.device("cuda", torch.cuda.current_device())
-    s = _status_of(device)
+    _status_of(device.index)
+    s = _status[device.index][1]
     torch.cuda.synchronize(device)
     bits = int(s.item())
     if bits:
@@ -76,7 +78,7 @@ class KvPool:
         if data.dtype not in _DTYPES or not data.is_cuda:
             raise _invalid("a KV pool holds bf16 or f16 values on a GPU")
         self.data = data
-        self.device, self.dtype = data.device, data.dtype
+        self.device, self.dtype, self.index = data.device, data.dtype, data.get_device()
         self.pages, self.layers, _, self.kv_heads, _, self.dim = data.shape
         self._c = _lib.KvPool(data.data_ptr(), self.pages, self.layers, self.kv_heads, self.dim, _DTYPES[data.dtype])
         self._ref = ctypes.addressof(self._c)
@@ -86,33 +88,45 @@ class KvPool:
         return cls(torch.zeros((pages, layers, 2, kv_heads, PAGE, dim), dtype=dtype, device=device))
 
 
-def _int(t, dtype, device, what, shape=None):
-    """The address of a contiguous device tensor of integers (or 32-bit floats)."""
-    if t.dtype is not dtype or t.device != device or not t.is_contiguous() or (shape is not None and t.shape != shape):
-        raise _invalid(f"{what} must be a contiguous {dtype} tensor on {device}"
-                       + (f" of shape {tuple(shape)}" if shape is not None else ""))
-    return t.data_ptr()
+# Calls of a few microseconds are the smallest cases' whole cost, so the checks below read each
+# attribute once and the stream's handle without building a Stream object.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
 
 
-def _rows(t, device, dtype, what):
+def _flat(t, dtype, index, what, count):
+    """The address of a contiguous [count] device tensor."""
+    if t.dtype is dtype and t.get_device() == index and t.dim() == 1 and t.shape[0] == count and t.is_contiguous():
+        return t.data_ptr()
+    raise _invalid(f"{what} must be a contiguous [{count}] tensor of {dtype} on cuda:{index}")
+
+
+def _table(t, dtype, index, what):
+    """The address of a contiguous [rows, columns] device tensor."""
+    if t.dtype is dtype and t.get_device() == index and t.dim() == 2 and t.is_contiguous():
+        return t.data_ptr()
+    raise _invalid(f"{what} must be a contiguous two-dimensional tensor of {dtype} on cuda:{index}")
+
+
+def _rows(t, index, dtype, what, shape=None):
     """The address and row stride of a [rows, heads, dim] tensor with adjacent heads."""
-    if t.dim() != 3 or t.dtype is not dtype or t.device != device:
-        raise _invalid(f"{what} must be a [rows, heads, dim] tensor of {dtype} on {device}")
+    if t.dtype is not dtype or t.get_device() != index or t.dim() != 3 or (shape is not None and t.shape != shape):
+        raise _invalid(f"{what} must be a [rows, heads, dim] tensor of {dtype} on cuda:{index}"
+                       + (f" of shape {tuple(shape)}" if shape is not None else ""))
     rows, heads, dim = t.shape
-    s = t.stride()
-    if t.numel() and (s[2] != 1 or (heads > 1 and s[1] != dim)):
+    step, head, one = t.stride()
+    if (one != 1 or (heads > 1 and head != dim)) and rows and heads and dim:
         raise _invalid(f"{what}: the heads of a row must be adjacent")
-    return t.data_ptr(), s[0] if rows > 1 and t.numel() else heads * dim
+    return t.data_ptr(), step if rows > 1 else heads * dim
 
 
-def _call(device, fn, *args):
+def _call(index, fn, *args):
     """fn(*args, status, stream) on the device's current stream."""
-    status = _status_of(device).data_ptr()
-    if torch.cuda.current_device() != device.index:
-        with torch.cuda.device(device):
-            rc = fn(*args, status, torch.cuda.current_stream(device).cuda_stream)
+    status = _status_of(index)
+    if torch.cuda.current_device() != index:
+        with torch.cuda.device(index):
+            rc = fn(*args, status, _raw_stream(index))
     else:
-        rc = fn(*args, status, torch.cuda.current_stream(device).cuda_stream)
+        rc = fn(*args, status, _raw_stream(index))
     if rc:
         _lib.check(rc)
 
@@ -125,10 +139,10 @@ def qk_rope_append(qkv, q_norm, k_norm, eps, cos, sin, positions, pool, layer, s
     slots [rows] int64, 64 * page + place, negative for a row whose K/V is not kept. Returns
     q [rows, heads, dim] (q_out when given); k_out [rows, kv, dim], when given, gets the rotated
     K as well. q_out and k_out may be the q and k parts of qkv."""
-    dev = pool.device
-    src, stride = _rows(qkv, dev, pool.dtype, "qkv")
+    dev, dtype, kv = pool.index, pool.dtype, pool.kv_heads
+    src, stride = _rows(qkv, dev, dtype, "qkv")
     rows, width, dim = qkv.shape
-    heads = width - 2 * pool.kv_heads
+    heads = width - 2 * kv
     if heads < 1 or dim != pool.dim:
         raise _invalid("qkv must be [rows, heads + 2 kv heads, dim] of the pool's kv heads and dim")
     if cos.shape != sin.shape or cos.dim() != 2 or cos.shape[1] != dim // 2:
@@ -136,21 +150,15 @@ def qk_rope_append(qkv, q_norm, k_norm, eps, cos, sin, positions, pool, layer, s
     if (q_norm is None) != (k_norm is None):
         raise _invalid("q_norm and k_norm go together")
     if q_out is None:
-        q_out = torch.empty((rows, heads, dim), dtype=qkv.dtype, device=dev)
-    elif q_out.shape != (rows, heads, dim):
-        raise _invalid("q_out must be [rows, heads, dim]")
-    qp, qs = _rows(q_out, dev, pool.dtype, "q_out")
-    kp, ks = 0, 0
-    if k_out is not None:
-        if k_out.shape != (rows, pool.kv_heads, dim):
-            raise _invalid("k_out must be [rows, kv heads, dim]")
-        kp, ks = _rows(k_out, dev, pool.dtype, "k_out")
+        q_out = qkv.new_empty((rows, heads, dim))
+    qp, qs = _rows(q_out, dev, dtype, "q_out", (rows, heads, dim))
+    kp, ks = (0, 0) if k_out is None else _rows(k_out, dev, dtype, "k_out", (rows, kv, dim))
     f32 = torch.float32
     _call(dev, _lib.lib().yue2_qk_rope_append, src, rows, heads, stride,
-          0 if q_norm is None else _int(q_norm, f32, dev, "q_norm", (dim,)),
-          0 if k_norm is None else _int(k_norm, f32, dev, "k_norm", (dim,)), eps, _int(cos, f32, dev, "cos"),
-          _int(sin, f32, dev, "sin"), cos.shape[0], _int(positions, torch.int32, dev, "positions", (rows,)), pool._ref, layer,
-          _int(slots, torch.int64, dev, "slots", (rows,)), qp, qs, kp if rows else 0, ks)
+          0 if q_norm is None else _flat(q_norm, f32, dev, "q_norm", dim),
+          0 if k_norm is None else _flat(k_norm, f32, dev, "k_norm", dim), eps, _table(cos, f32, dev, "cos"),
+          _table(sin, f32, dev, "sin"), cos.shape[0], _flat(positions, torch.int32, dev, "positions", rows), pool._ref, layer,
+          _flat(slots, torch.int64, dev, "slots", rows), qp, qs, kp if rows else 0, ks)
     return q_out
 
 
@@ -161,25 +169,25 @@ def attention_packed(q, k, v, cu, causal=True, scale=None, out=None):
     or all of it with causal=False. scale: 1 / sqrt(dim) by default. Rows outside
     [cu[0], cu[-1]) of `out` are left as they were (undefined when `out` is None). bf16 or
     f16, dim 64 or 128; strided rows are fine."""
-    dev, dtype = q.device, q.dtype
-    if dtype not in _DTYPES or not q.is_cuda:
+    dev, dtype = q.get_device(), q.dtype
+    code = _DTYPES.get(dtype)
+    if code is None or dev < 0:
         raise _invalid("attention takes bf16 or f16 tensors on a GPU")
     qp, qs = _rows(q, dev, dtype, "q")
     kp, ks = _rows(k, dev, dtype, "k")
-    vp, vs = _rows(v, dev, dtype, "v")
     tokens, heads, dim = q.shape
     kv = k.shape[1]
-    if k.shape != v.shape or k.shape[0] != tokens or k.shape[2] != dim:
+    vp, vs = _rows(v, dev, dtype, "v", (tokens, kv, dim))
+    if k.shape[0] != tokens or k.shape[2] != dim:
         raise _invalid("k and v must be [tokens, kv heads, dim] of q's tokens and dim")
     if out is None:
-        out = torch.empty((tokens, heads, dim), dtype=dtype, device=dev)
-    elif out.shape != q.shape:
-        raise _invalid("out must have q's shape")
-    op, os_ = _rows(out, dev, dtype, "out")
+        out = q.new_empty((tokens, heads, dim))
+    op, os_ = _rows(out, dev, dtype, "out", (tokens, heads, dim))
     if cu.dim() != 1 or cu.shape[0] < 1:
         raise _invalid("cu must be [seqs + 1]")
-    _call(dev, _lib.lib().yue2_attention_packed, qp, kp, vp, op, _int(cu, torch.int32, dev, "cu"), cu.shape[0] - 1, tokens,
-          heads, kv, dim, qs, ks, vs, os_, _DTYPES[dtype], 1 if causal else 0, 1 / math.sqrt(dim) if scale is None else scale)
+    seqs = cu.shape[0] - 1
+    _call(dev, _lib.lib().yue2_attention_packed, qp, kp, vp, op, _flat(cu, torch.int32, dev, "cu", seqs + 1), seqs, tokens,
+          heads, kv, dim, qs, ks, vs, os_, code, 1 if causal else 0, dim ** -0.5 if scale is None else scale)
     return out
 
 
@@ -191,25 +199,22 @@ def attention_tree(q, pool, layer, table, context, cu, mask=None, scale=None, ou
     (int64: a node's ancestors and itself); mask None: all up to itself, so that one row per
     sequence is an ordinary decode step. A row that sees nothing gets zeros; rows outside
     [cu[0], cu[-1]) of `out` are left as they were (undefined when `out` is None)."""
-    dev = pool.device
-    qp, qs = _rows(q, dev, pool.dtype, "q")
+    dev, dtype, i32 = pool.index, pool.dtype, torch.int32
+    qp, qs = _rows(q, dev, dtype, "q")
     rows, heads, dim = q.shape
     if dim != pool.dim:
         raise _invalid("q must have the pool's dim")
     if out is None:
-        out = torch.empty((rows, heads, dim), dtype=q.dtype, device=dev)
-    elif out.shape != q.shape:
-        raise _invalid("out must have q's shape")
-    op, os_ = _rows(out, dev, pool.dtype, "out")
-    if table.dim() != 2:
-        raise _invalid("table must be [seqs, pages]")
+        out = q.new_empty((rows, heads, dim))
+    op, os_ = _rows(out, dev, dtype, "out", (rows, heads, dim))
+    tp = _table(table, i32, dev, "table")
     seqs, pages = table.shape
     L = _lib.lib()
     need = L.yue2_attention_tree_workspace(rows, heads, seqs, pages, pool._ref)
-    work = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    _call(dev, L.yue2_attention_tree, qp, rows, heads, qs, pool._ref, layer, _int(table, torch.int32, dev, "table"), seqs, pages,
-          _int(context, torch.int32, dev, "context", (seqs,)), _int(cu, torch.int32, dev, "cu", (seqs + 1,)),
-          0 if mask is None else _int(mask, torch.int64, dev, "mask", (rows,)), 1 / math.sqrt(dim) if scale is None else scale,
+    work = q.new_empty((need + 1) // 2) if need else None  # 16-bit values
+    _call(dev, L.yue2_attention_tree, qp, rows, heads, qs, pool._ref, layer, tp, seqs, pages,
+          _flat(context, i32, dev, "context", seqs), _flat(cu, i32, dev, "cu", seqs + 1),
+          0 if mask is None else _flat(mask, torch.int64, dev, "mask", rows), dim ** -0.5 if scale is None else scale,
           op, os_, work.data_ptr() if need else 0, need)
     return out
 
@@ -217,10 +222,9 @@ def attention_tree(q, pool, layer, table, context, cu, mask=None, scale=None, ou
 def kv_copy(pool, src, dst, count=None):
     """Positions [0, count[i]) (all 64 when count is None) of page src[i] to page dst[i], in
     every layer; int32 [n] each. The dst pages are distinct and none of them is a src page."""
-    n = src.shape[0]
-    _call(pool.device, _lib.lib().yue2_kv_copy, pool._ref, _int(src, torch.int32, pool.device, "src", (n,)),
-          _int(dst, torch.int32, pool.device, "dst", (n,)),
-          0 if count is None else _int(count, torch.int32, pool.device, "count", (n,)), n)
+    dev, i32, n = pool.index, torch.int32, src.shape[0]
+    _call(dev, _lib.lib().yue2_kv_copy, pool._ref, _flat(src, i32, dev, "src", n), _flat(dst, i32, dev, "dst", n),
+          0 if count is None else _flat(count, i32, dev, "count", n), n)
 
 
 def kv_gather(pool, src_table, dst_table, begin, cu, keep):
@@ -230,13 +234,16 @@ def kv_gather(pool, src_table, dst_table, begin, cu, keep):
     path of a drafted tree, dropping positions), and the pages written are the sequence's
     own. Otherwise into the pages of dst_table, none of which the call reads; keep in any
     order. Tables int32 [seqs, pages], begin int32 [seqs], cu int32 [seqs + 1], keep int32."""
-    dev, i32 = pool.device, torch.int32
-    if src_table.dim() != 2 or (dst_table is not None and (dst_table.dim() != 2 or dst_table.shape[0] != src_table.shape[0])):
-        raise _invalid("page tables must be [seqs, pages] of the same sequences")
-    seqs = src_table.shape[0]
+    dev, i32 = pool.index, torch.int32
+    sp = _table(src_table, i32, dev, "src_table")
+    seqs, pages = src_table.shape
+    dp, dst_pages = 0, 0
+    if dst_table is not None:
+        dp, dst_pages = _table(dst_table, i32, dev, "dst_table"), dst_table.shape[1]
+        if dst_table.shape[0] != seqs:
+            raise _invalid("src_table and dst_table must hold the same sequences")
     if keep.dim() != 1:
         raise _invalid("keep must be one list")
-    _call(dev, _lib.lib().yue2_kv_gather, pool._ref, _int(src_table, i32, dev, "src_table"), src_table.shape[1],
-          0 if dst_table is None else _int(dst_table, i32, dev, "dst_table"), 0 if dst_table is None else dst_table.shape[1],
-          _int(begin, i32, dev, "begin", (seqs,)), _int(cu, i32, dev, "cu", (seqs + 1,)), _int(keep, i32, dev, "keep"), seqs,
-          keep.shape[0])
+    total = keep.shape[0]
+    _call(dev, _lib.lib().yue2_kv_gather, pool._ref, sp, pages, dp, dst_pages, _flat(begin, i32, dev, "begin", seqs),
+          _flat(cu, i32, dev, "cu", seqs + 1), _flat(keep, i32, dev, "keep", total), seqs, total)
