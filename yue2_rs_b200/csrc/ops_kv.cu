@@ -11,10 +11,11 @@ namespace {
 
 // ------------------------------------------------------------------ QK norm + rotation + append
 // y = x * rsqrt(mean(x^2) + eps) * gain, then (a, b) = (y_i, y_{i + D/2}) becomes
-// (a cos - b sin, b cos + a sin). One head is D/8 lanes of 8 elements (one 16-byte load and
-// store each); the partner i + D/2 of an element is D/16 lanes away, so a shuffle brings it.
-// One CTA per row: its groups of D/8 lanes take the row's heads in turn and keep the
-// row's cos and sin in registers.
+// (a cos - b sin, b cos + a sin). One head is D/8 lanes, each with 4 elements of the first
+// half and their 4 partners of the second (two 8-byte loads and stores), so that the
+// rotation needs no exchange between lanes: the arithmetic, not only the bytes, bounds this
+// pass. One CTA per row: its groups of D/8 lanes take the row's heads in turn and keep the
+// row's cos and sin and the gains in registers.
 struct AppendParams {
   const uint16_t* qkv;
   uint16_t *q_out, *k_out;
@@ -28,9 +29,17 @@ struct AppendParams {
   float eps;
 };
 
-constexpr int kAppendThreads = 256;
+constexpr int kAppendThreads = 64;  // 8,192 rows of 40 heads: 40.9 us; 128 threads 45.4, 256 51.3
 
-template <int D, bool F16>
+Y2_DEV void load4(const float* p, float (&v)[4]) {
+  const float4 a = *reinterpret_cast<const float4*>(p);
+  v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+}
+
+// UNROLL heads of a group are loaded before the row's position, which the loads of cos and sin
+// wait for, is known. The gains stay in registers: read again for every head they kept L1
+// 80% busy and took a third of the pass.
+template <int D, bool F16, int UNROLL>
 __global__ void __launch_bounds__(kAppendThreads) qk_rope_append_kernel(const AppendParams p) {
   constexpr int L = D / 8;                     // lanes per head
   constexpr int GROUPS = kAppendThreads / L;   // heads in flight
@@ -38,63 +47,100 @@ __global__ void __launch_bounds__(kAppendThreads) qk_rope_append_kernel(const Ap
   const int group = threadIdx.x / L, l = threadIdx.x % L;
   const int kv = p.pool.kv, total = p.heads + 2 * kv;
   const int pos = p.positions[row];
-  if (pos < 0 || pos >= p.table_rows) {
-    if (threadIdx.x == 0) status_or(p.status, YUE2_STATUS_RANGE);
-    return;
-  }
   const long long slot = p.slots[row];
+  const uint16_t* src = p.qkv + row * p.qkv_stride + l * 4;
+  float c[4], s[4], gq[8], gk[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) gq[e] = gk[e] = 1.f;
+  if (p.q_norm) {
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      float a[4], b[4];
+      load4(p.q_norm + half * (D / 2) + l * 4, a);
+      load4(p.k_norm + half * (D / 2) + l * 4, b);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) gq[4 * half + e] = a[e], gk[4 * half + e] = b[e];
+    }
+  }
+  const bool inside = pos >= 0 && pos < p.table_rows;
   const bool store = slot >= 0 && (slot >> kPageLog2) < p.pool.pages;
-  if (slot >= 0 && !store && threadIdx.x == 0) status_or(p.status, YUE2_STATUS_PAGE);
-  uint16_t* page = p.pool.base + (store ? (slot >> kPageLog2) * p.pool.page_stride : 0);
-  const long long place = (slot & (kPageTokens - 1)) * D + l * 8;
-  const int half = (l % (L / 2)) * 8;
-  float c[8], s[8];
-  {
-    const float* ct = p.cos + (long long)pos * (D / 2) + half;
-    const float* st = p.sin + (long long)pos * (D / 2) + half;
+  uint16_t* page = p.pool.base + (store ? (slot >> kPageLog2) * p.pool.page_stride : 0) +
+                   (long long)p.layer * 2 * kv * (kPageTokens * D) + (slot & (kPageTokens - 1)) * D + l * 4;
+  for (int h0 = group; h0 - group < total; h0 += GROUPS * UNROLL) {
+    uint2 lo[UNROLL], hi[UNROLL];
 #pragma unroll
-    for (int e = 0; e < 8; e += 4) {
-      const float4 a = *reinterpret_cast<const float4*>(ct + e), b = *reinterpret_cast<const float4*>(st + e);
-      c[e] = a.x, c[e + 1] = a.y, c[e + 2] = a.z, c[e + 3] = a.w;
-      s[e] = b.x, s[e + 1] = b.y, s[e + 2] = b.z, s[e + 3] = b.w;
+    for (int u = 0; u < UNROLL; ++u) {
+      const int h = h0 + u * GROUPS;
+      lo[u] = hi[u] = make_uint2(0, 0);
+      if (h < total) {
+        lo[u] = *reinterpret_cast<const uint2*>(src + (long long)h * D);
+        hi[u] = *reinterpret_cast<const uint2*>(src + (long long)h * D + D / 2);
+      }
+    }
+    if (h0 == group) {
+      if (!inside || (slot >= 0 && !store)) {
+        if (threadIdx.x == 0) status_or(p.status, inside ? YUE2_STATUS_PAGE : YUE2_STATUS_RANGE);
+        if (!inside) return;
+      }
+      load4(p.cos + (long long)pos * (D / 2) + l * 4, c);
+      load4(p.sin + (long long)pos * (D / 2) + l * 4, s);
+    }
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      const int h = h0 + u * GROUPS;
+      const bool is_q = h < p.heads, is_v = h >= p.heads + kv;
+      const bool copies = __all_sync(0xffffffffu, is_v);  // a warp of value heads only copies
+      if (!copies) {
+        float a[4] = {lo16<F16>(lo[u].x), hi16<F16>(lo[u].x), lo16<F16>(lo[u].y), hi16<F16>(lo[u].y)};
+        float b[4] = {lo16<F16>(hi[u].x), hi16<F16>(hi[u].x), lo16<F16>(hi[u].y), hi16<F16>(hi[u].y)};
+        if (p.q_norm) {
+          float ss = 0.f;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) ss = fmaf(b[e], b[e], fmaf(a[e], a[e], ss));
+#pragma unroll
+          for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+          const float scale = rsqrtf(ss * (1.0f / D) + p.eps);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            a[e] *= scale * (is_q ? gq[e] : gk[e]);
+            b[e] *= scale * (is_q ? gq[4 + e] : gk[4 + e]);
+          }
+        }
+        float y[4], z[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          y[e] = a[e] * c[e] - b[e] * s[e];
+          z[e] = b[e] * c[e] + a[e] * s[e];
+        }
+        if (!is_v) {
+          lo[u] = make_uint2(pack16<F16>(y[0], y[1]), pack16<F16>(y[2], y[3]));
+          hi[u] = make_uint2(pack16<F16>(z[0], z[1]), pack16<F16>(z[2], z[3]));
+        }
+      }
+      if (h >= total) continue;
+      auto put = [&](uint16_t* to) {
+        *reinterpret_cast<uint2*>(to) = lo[u];
+        *reinterpret_cast<uint2*>(to + D / 2) = hi[u];
+      };
+      if (is_q) {
+        put(p.q_out + row * p.q_stride + (long long)h * D + l * 4);
+      } else {
+        const int j = h - p.heads;  // K heads then V heads, as the pool's blocks of a layer
+        if (!is_v && p.k_out) put(p.k_out + row * p.k_stride + (long long)j * D + l * 4);
+        if (store) put(page + (long long)j * (kPageTokens * D));
+      }
     }
   }
-  const uint16_t* src = p.qkv + row * p.qkv_stride + l * 8;
-  for (int h0 = 0; h0 < total; h0 += GROUPS) {
-    const int h = h0 + group;
-    const bool live = h < total;
-    const uint4 w = live ? *reinterpret_cast<const uint4*>(src + (long long)h * D) : make_uint4(0, 0, 0, 0);
-    float x[8];
-    unpack8<F16>(w, x);
-    const bool is_q = h < p.heads, is_v = h >= p.heads + kv;
-    if (p.q_norm) {
-      float ss = 0.f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
-#pragma unroll
-      for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      const float scale = 1.0f / sqrtf(ss / (float)D + p.eps);
-      const float* gain = (is_q ? p.q_norm : p.k_norm) + l * 8;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] *= scale * gain[e];
-    }
-    float y[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float other = __shfl_xor_sync(0xffffffffu, x[e], L / 2);
-      y[e] = l < L / 2 ? x[e] * c[e] - other * s[e] : x[e] * c[e] + other * s[e];
-    }
-    if (!live) continue;
-    const uint4 r = is_v ? w : pack8<F16>(y);
-    if (is_q) {
-      *reinterpret_cast<uint4*>(p.q_out + row * p.q_stride + (long long)h * D + l * 8) = r;
-    } else {
-      const int j = h - p.heads;  // K heads then V heads, as the pool's blocks of a layer
-      if (!is_v && p.k_out) *reinterpret_cast<uint4*>(p.k_out + row * p.k_stride + (long long)j * D + l * 8) = r;
-      if (store)
-        *reinterpret_cast<uint4*>(page + ((long long)p.layer * 2 * kv + j) * (kPageTokens * D) + place) = r;
-    }
-  }
+}
+
+template <int D, bool F16>
+void launch_append(const AppendParams& p, unsigned rows, cudaStream_t st) {
+  constexpr int GROUPS = kAppendThreads / (D / 8);
+  const int rounds = (p.heads + 2 * p.pool.kv + GROUPS - 1) / GROUPS;
+  if (rounds <= 1) qk_rope_append_kernel<D, F16, 1><<<rows, kAppendThreads, 0, st>>>(p);
+  else if (rounds == 2) qk_rope_append_kernel<D, F16, 2><<<rows, kAppendThreads, 0, st>>>(p);
+  else if (rounds == 3) qk_rope_append_kernel<D, F16, 3><<<rows, kAppendThreads, 0, st>>>(p);
+  else qk_rope_append_kernel<D, F16, 5><<<rows, kAppendThreads, 0, st>>>(p);
 }
 
 // ------------------------------------------------------------------ page copy
@@ -204,7 +250,8 @@ int yue2_qk_rope_append(const void* qkv, uint64_t rows, uint64_t heads, uint64_t
   if ((rc = check_rows(qkv, rows, heads + 2 * pool->kv, pool->dim, qkv_stride, "qkv"))) return rc;
   if ((rc = check_rows(q_out, rows, heads, pool->dim, q_stride, "q_out"))) return rc;
   if (k_out && (rc = check_rows(k_out, rows, pool->kv, pool->dim, k_stride, "k_out"))) return rc;
-  if (!q_norm != !k_norm) return fail(YUE2_ERR_INVALID, "q_norm and k_norm go together");
+  if (!q_norm != !k_norm || !aligned16(q_norm) || !aligned16(k_norm))
+    return fail(YUE2_ERR_INVALID, "q_norm and k_norm go together and are 16-byte aligned");
   if (rows && (!positions || !slots || !cos || !sin || !aligned16(cos) || !aligned16(sin)))
     return fail(YUE2_ERR_INVALID, "positions, slots and 16-byte aligned cos and sin tables are needed");
   if (!(eps >= 0.f)) return fail(YUE2_ERR_INVALID, "eps must not be negative");
@@ -227,12 +274,11 @@ int yue2_qk_rope_append(const void* qkv, uint64_t rows, uint64_t heads, uint64_t
   p.layer = (int)layer;
   p.eps = eps;
   const bool f16 = pool->dtype == YUE2_DTYPE_F16;
-  const dim3 grid((unsigned)rows);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-#define Y2_APPEND(DD)                                                              \
-  case DD:                                                                         \
-    if (f16) qk_rope_append_kernel<DD, true><<<grid, kAppendThreads, 0, st>>>(p);  \
-    else qk_rope_append_kernel<DD, false><<<grid, kAppendThreads, 0, st>>>(p);     \
+#define Y2_APPEND(DD)                                               \
+  case DD:                                                          \
+    if (f16) launch_append<DD, true>(p, (unsigned)rows, st);        \
+    else launch_append<DD, false>(p, (unsigned)rows, st);           \
     break;
   switch (p.pool.dim) {
     Y2_APPEND(64)
