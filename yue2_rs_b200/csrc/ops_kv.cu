@@ -165,67 +165,74 @@ __global__ void __launch_bounds__(kMoveThreads) kv_copy_kernel(PoolView pool, co
 }
 
 // ------------------------------------------------------------------ position moves
-// CTA (block b, sequence s, share z): rows of dim * 2 bytes of one block, in chunks of
-// kMoveRows positions in list order. In place, keep is strictly increasing and keep[i] >= begin + i, so a
-// write of chunk c lands on positions that no later chunk reads; within a chunk every read
-// precedes every write (barrier). Out of place nothing read is written and the chunks of a
-// sequence go to several CTAs.
+// A warp moves rows of dim * 2 bytes, kMoveRows of them at a time in list order, in a few of the
+// page's blocks: the list and the page tables are looked up once for all of those. In place,
+// keep is strictly increasing and keep[i] >= begin + i, so a write lands on no position that a
+// later entry reads; an earlier entry's read is of the same or an earlier group, which the
+// warp has finished (or orders with __syncwarp) before it writes. Out of place nothing read is
+// written and the groups of a list go to several CTAs.
 struct GatherParams {
   PoolView pool;
   const int32_t *src_table, *dst_table, *begin, *cu, *keep;
   int32_t* status;
   long long src_pages, dst_pages, total;
+  int per_warp;  // blocks of a page that a warp takes
 };
+constexpr int kMoveUnroll = 8;  // rows in flight per lane
 
 template <int D>
 __global__ void __launch_bounds__(kMoveThreads) kv_gather_kernel(const GatherParams p) {
-  constexpr int L = D / 8;                     // lanes per row
-  constexpr int RP = kMoveThreads / L;         // rows per pass
-  constexpr int U = 4;                         // passes in flight
-  const int s = blockIdx.y;
+  constexpr int L = D / 8;                         // lanes per row
+  constexpr int ROWS = 32 / L * kMoveUnroll;       // rows of a group
+  const int s = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int block0 = (blockIdx.x * (kMoveThreads / 32) + warp) * p.per_warp, block1 = min(block0 + p.per_warp, p.pool.blocks);
   const bool in_place = p.dst_table == nullptr;
   const int first = p.cu[s], last = p.cu[s + 1], begin = p.begin[s];
-  const bool lead = threadIdx.x == 0 && blockIdx.x == 0;
+  const bool reports = block0 == 0;  // one warp tells what is wrong with an entry
   if (first < 0 || last < first || last > p.total || begin < 0) {
-    if (lead && blockIdx.z == 0) status_or(p.status, YUE2_STATUS_RANGE);
+    if (reports && lane == 0 && blockIdx.z == 0) status_or(p.status, YUE2_STATUS_RANGE);
     return;
   }
   const int32_t* src_row = p.src_table + (long long)s * p.src_pages;
   const int32_t* dst_row = in_place ? src_row : p.dst_table + (long long)s * p.dst_pages;
   const long long dst_pages = in_place ? p.src_pages : p.dst_pages;
-  const long long block = (long long)blockIdx.x * kPageTokens * D;
-  const int sub = threadIdx.x / L, l = threadIdx.x % L;
-  const int n = last - first;
-  const int step = RP * U * gridDim.z;
-  for (int c0 = RP * U * blockIdx.z; c0 < n; c0 += step) {
-    uint4 v[U];
-    uint16_t* to[U];
+  const int sub = lane / L, l = lane % L, n = last - first;
+  for (int c0 = ROWS * blockIdx.z; c0 < n; c0 += ROWS * gridDim.z) {
+    const uint16_t* from[kMoveUnroll];
+    uint16_t* to[kMoveUnroll];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int i = c0 + u * RP + sub;
+    for (int u = 0; u < kMoveUnroll; ++u) {
+      const int i = c0 + u * (32 / L) + sub;
       to[u] = nullptr;
+      from[u] = nullptr;
       if (i >= n) continue;
-      const long long from = p.keep[first + i], dest = (long long)begin + i;
+      const long long x = p.keep[first + i], y = (long long)begin + i;
       // the order that in-place moves rely on, for this entry and the one before it
-      const bool order = !in_place || (from >= dest && (i == 0 || p.keep[first + i - 1] < from));
-      if (from < 0 || (from >> kPageLog2) >= p.src_pages || (dest >> kPageLog2) >= dst_pages || !order) {
-        if (l == 0 && blockIdx.x == 0) status_or(p.status, YUE2_STATUS_RANGE);
+      const bool order = !in_place || (x >= y && (i == 0 || p.keep[first + i - 1] < x));
+      if (x < 0 || (x >> kPageLog2) >= p.src_pages || (y >> kPageLog2) >= dst_pages || !order) {
+        if (reports && l == 0) status_or(p.status, YUE2_STATUS_RANGE);
         continue;
       }
-      const long long a = src_row[from >> kPageLog2], b = dst_row[dest >> kPageLog2];
+      const long long a = src_row[x >> kPageLog2], b = dst_row[y >> kPageLog2];
       if (a < 0 || a >= p.pool.pages || b < 0 || b >= p.pool.pages) {
-        if (l == 0 && blockIdx.x == 0) status_or(p.status, YUE2_STATUS_PAGE);
+        if (reports && l == 0) status_or(p.status, YUE2_STATUS_PAGE);
         continue;
       }
-      v[u] = *reinterpret_cast<const uint4*>(p.pool.base + a * p.pool.page_stride + block +
-                                             (from & (kPageTokens - 1)) * D + l * 8);
-      to[u] = p.pool.base + b * p.pool.page_stride + block + (dest & (kPageTokens - 1)) * D + l * 8;
+      from[u] = p.pool.base + a * p.pool.page_stride + (x & (kPageTokens - 1)) * D + l * 8;
+      to[u] = p.pool.base + b * p.pool.page_stride + (y & (kPageTokens - 1)) * D + l * 8;
     }
-    if (in_place) __syncthreads();
+    for (int block = block0; block < block1; ++block) {
+      const long long off = (long long)block * (kPageTokens * D);
+      uint4 v[kMoveUnroll];
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (to[u]) *reinterpret_cast<uint4*>(to[u]) = v[u];
-    if (in_place) __syncthreads();
+      for (int u = 0; u < kMoveUnroll; ++u)
+        if (to[u]) v[u] = *reinterpret_cast<const uint4*>(from[u] + off);
+      __syncwarp();
+#pragma unroll
+      for (int u = 0; u < kMoveUnroll; ++u)
+        if (to[u]) *reinterpret_cast<uint4*>(to[u] + off) = v[u];
+      __syncwarp();
+    }
   }
 }
 
@@ -323,9 +330,14 @@ int yue2_kv_gather(const Yue2KvPool* pool, const int32_t* src_table, uint64_t sr
   p.src_pages = (long long)src_pages;
   p.dst_pages = (long long)dst_pages;
   p.total = (long long)total;
-  // out of place: one CTA per 64 positions of the average list, at most 64 per (block, sequence)
-  const uint64_t shares = dst_table ? std::min<uint64_t>(64, (total / seqs + 63) / 64) : 1;
-  const dim3 grid((unsigned)p.pool.blocks, (unsigned)seqs, (unsigned)std::max<uint64_t>(1, shares));
+  // Out of place: a warp group per group of rows of the average list, at most 256 shares. A warp
+  // takes several blocks as long as that leaves about 16 warps for each SM.
+  const uint64_t rows = 256 / pool->dim * kMoveUnroll;
+  const uint64_t shares = dst_table ? std::min<uint64_t>(256, (total / seqs + rows - 1) / rows) : 1;
+  const unsigned z = (unsigned)std::max<uint64_t>(1, shares);
+  p.per_warp = (int)std::max<uint64_t>(1, std::min<uint64_t>(4, (uint64_t)p.pool.blocks * seqs * z / 2368));
+  const int per_cta = kMoveThreads / 32 * p.per_warp;
+  const dim3 grid((unsigned)((p.pool.blocks + per_cta - 1) / per_cta), (unsigned)seqs, z);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   switch (p.pool.dim) {
     case 64: kv_gather_kernel<64><<<grid, kMoveThreads, 0, st>>>(p); break;
