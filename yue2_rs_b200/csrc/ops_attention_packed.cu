@@ -58,7 +58,7 @@ struct Layout {
   static constexpr int BARS = 2 * SLOTS + 2 * kUnits + 2 + 8 + 1;
   static constexpr int OFF_UNIT = OFF_BAR + BARS * 8;
   static constexpr int OFF_MISC = OFF_UNIT + kUnits * (int)sizeof(Unit);
-  static constexpr int BYTES = OFF_MISC + 16 + 1024;
+  static constexpr int BYTES = OFF_MISC + 16;
 };
 
 struct Seq {
@@ -136,8 +136,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                             const __grid_constant__ CUtensorMap mv, const PackedArgs a) {
   using L = Layout<D>;
   constexpr int SLOTS = L::SLOTS, TILE = L::TILE;
-  extern __shared__ unsigned char smem_raw[];
-  unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  extern __shared__ __align__(1024) unsigned char smem[];
   uint64_t* bar = (uint64_t*)(smem + L::OFF_BAR);
   uint64_t *kv_full = bar, *kv_empty = bar + SLOTS, *unit_full = kv_empty + SLOTS, *unit_empty = unit_full + kUnits;
   uint64_t *q_full = unit_empty + kUnits, *q_empty = q_full + 1, *drain = q_empty + 1;

@@ -107,7 +107,7 @@ struct Layout {
   static constexpr int OFF_UNIT = OFF_BAR + BARS * 8;
   static constexpr int OFF_ML = OFF_UNIT + kUnits * (int)sizeof(Unit);
   static constexpr int OFF_MISC = OFF_ML + kRows * 8;
-  static constexpr int BYTES = OFF_MISC + 16 + 1024;
+  static constexpr int BYTES = OFF_MISC + 16;
 };
 
 // A unit's sides. One side of nodes: both hold it and side s takes tiles t0 + s, t0 + s + 2, ..
@@ -131,8 +131,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     attention_tree_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mkv, const TreeArgs a) {
   using L = Layout<D>;
   constexpr int SLOTS = L::SLOTS, TILE = L::TILE;
-  extern __shared__ unsigned char smem_raw[];
-  unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  extern __shared__ __align__(1024) unsigned char smem[];
   uint64_t* bar = (uint64_t*)(smem + L::OFF_BAR);
   uint64_t *kv_full = bar, *kv_empty = bar + SLOTS, *unit_full = kv_empty + SLOTS, *unit_empty = unit_full + kUnits;
   uint64_t *q_full = unit_empty + kUnits, *q_empty = q_full + 1, *drain = q_empty + 1;
@@ -421,8 +420,20 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else {
     // ---------------------------------------------------------------- shares and page loads
     const bool report = blockIdx.x == 0;
-    long long sum = 0;
-    for (int s = lane; s < a.seqs; s += 32) sum += seq_length(a, seq_work(a, s, report));
+    // lane l keeps sequence l (most calls have no more), so that the walk needs no second look
+    const SeqWork lane_work = lane < a.seqs ? seq_work(a, lane, report) : SeqWork{0, 0, 0, 0, 0};
+    auto work_of = [&](int s) {
+      if (s >= 32) return seq_work(a, s, false);
+      SeqWork w;
+      w.first = __shfl_sync(0xffffffffu, lane_work.first, s);
+      w.n = __shfl_sync(0xffffffffu, lane_work.n, s);
+      w.tiles = __shfl_sync(0xffffffffu, lane_work.tiles, s);
+      w.parts = __shfl_sync(0xffffffffu, lane_work.parts, s);
+      w.ctx = __shfl_sync(0xffffffffu, lane_work.ctx, s);
+      return w;
+    };
+    long long sum = seq_length(a, lane_work);
+    for (int s = lane + 32; s < a.seqs; s += 32) sum += seq_length(a, seq_work(a, s, report));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     const bool fits = sum < INT32_MAX;
@@ -436,7 +447,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     int seq = 0, before = 0;
     if (at < end) {
       for (;; seq += 32) {
-        const int own = seq + lane < a.seqs ? seq_length(a, seq_work(a, seq + lane, false)) : 0;
+        const int own = seq == 0 ? seq_length(a, lane_work)
+                        : seq + lane < a.seqs ? seq_length(a, seq_work(a, seq + lane, false)) : 0;
         int upto = own;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -454,7 +466,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     SeqWork w = {0, 0, 0, 0, 0};
-    if (at < end) w = seq_work(a, seq, false);
+    if (at < end) w = work_of(seq);
     int length = item_length(w), total = seq_length(a, w);
     uint32_t kv_count = 0, q_count = 0;
     bool ok = true;
@@ -463,7 +475,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       while (at < end) {
         while (at >= before + total) {
           before += total;
-          w = seq_work(a, ++seq, false);
+          w = work_of(++seq);
           length = item_length(w), total = seq_length(a, w);
         }
         const int item = (at - before) / length, item0 = before + item * length;
@@ -547,9 +559,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // Rows of items that were cut: the partial results of their shares, in tile order. A CTA takes
-// eight heads of a row, a warp each.
+// eight heads of a row, a warp each. Its 40 registers a thread and little shared memory fit beside an
+// attention CTA, so that it is set up before that ends.
 template <int D, bool F16>
-__global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(const TreeArgs a) {
+__global__ void __launch_bounds__(kMergeThreads, 6) tree_merge_kernel(const TreeArgs a) {
   __shared__ int s_seq;
   __shared__ long long s_sum[2][kMergeThreads / 32];
   const int row = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -573,14 +586,14 @@ __global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(const TreeArg
   __syncthreads();
   long long all = 0, before = 0;
   for (int i = 0; i < kMergeThreads / 32; ++i) all += s_sum[0][i], before += s_sum[1][i];
-  pdl_wait();  // by every thread, whatever its row
-  if (seq == a.seqs || h >= a.heads || all >= INT32_MAX) return;
-  const SeqWork w = seq_work(a, seq, false);
-  const Shares shares(a, (int)all);
+  const bool some = seq < a.seqs && h < a.heads && all < INT32_MAX;
+  const SeqWork w = some ? seq_work(a, seq, false) : SeqWork{0, 0, 0, 0, 0};
+  const Shares shares(a, some ? (int)all : 0);
   const int node = row - w.first, block = node / (2 * a.nodes), length = item_length(w);
-  const int x0 = (int)before + ((h / a.group) * w.parts + block) * length;
-  const int c0 = shares.owner(x0 + kItemCost), c1 = shares.owner(x0 + length - 1);
-  if (c0 == c1) return;  // finished by its CTA
+  const int x0 = some ? (int)before + ((h / a.group) * w.parts + block) * length : 0;
+  const int c0 = some ? shares.owner(x0 + kItemCost) : 0, c1 = some ? shares.owner(x0 + length - 1) : 0;
+  pdl_wait();             // by every thread, whatever its row
+  if (c0 == c1) return;  // nothing to do, or finished by its CTA
   constexpr int E = D / 32;
   const float2* stats = reinterpret_cast<const float2*>(a.part + 2ll * a.ctas * a.slot_rows * D);
   const long long r = (node - block * 2 * a.nodes) * a.group + h % a.group;

@@ -82,6 +82,16 @@ class KvPool:
         self.pages, self.layers, _, self.kv_heads, _, self.dim = data.shape
         self._c = _lib.KvPool(data.data_ptr(), self.pages, self.layers, self.kv_heads, self.dim, _DTYPES[data.dtype])
         self._ref = ctypes.addressof(self._c)
+        self._sizes = {}  # bytes of the tree attention's workspace by (rows, heads, seqs, pages)
+
+    def _workspace(self, *shape):
+        need = self._sizes.get(shape)
+        if need is None:
+            with torch.cuda.device(self.index):
+                need = _lib.lib().yue2_attention_tree_workspace(*shape, self._ref)
+            if len(self._sizes) < 4096:
+                self._sizes[shape] = need
+        return need
 
     @classmethod
     def zeros(cls, pages, layers, kv_heads, dim, dtype=torch.bfloat16, device="cuda"):
@@ -151,7 +161,9 @@ def qk_rope_append(qkv, q_norm, k_norm, eps, cos, sin, positions, pool, layer, s
         raise _invalid("q_norm and k_norm go together")
     if q_out is None:
         q_out = qkv.new_empty((rows, heads, dim))
-    qp, qs = _rows(q_out, dev, dtype, "q_out", (rows, heads, dim))
+        qp, qs = q_out.data_ptr(), heads * dim
+    else:
+        qp, qs = _rows(q_out, dev, dtype, "q_out", (rows, heads, dim))
     kp, ks = (0, 0) if k_out is None else _rows(k_out, dev, dtype, "k_out", (rows, kv, dim))
     f32 = torch.float32
     _call(dev, _lib.lib().yue2_qk_rope_append, src, rows, heads, stride,
@@ -182,7 +194,9 @@ def attention_packed(q, k, v, cu, causal=True, scale=None, out=None):
         raise _invalid("k and v must be [tokens, kv heads, dim] of q's tokens and dim")
     if out is None:
         out = q.new_empty((tokens, heads, dim))
-    op, os_ = _rows(out, dev, dtype, "out", (tokens, heads, dim))
+        op, os_ = out.data_ptr(), heads * dim
+    else:
+        op, os_ = _rows(out, dev, dtype, "out", (tokens, heads, dim))
     if cu.dim() != 1 or cu.shape[0] < 1:
         raise _invalid("cu must be [seqs + 1]")
     seqs = cu.shape[0] - 1
@@ -206,11 +220,13 @@ def attention_tree(q, pool, layer, table, context, cu, mask=None, scale=None, ou
         raise _invalid("q must have the pool's dim")
     if out is None:
         out = q.new_empty((rows, heads, dim))
-    op, os_ = _rows(out, dev, dtype, "out", (rows, heads, dim))
+        op, os_ = out.data_ptr(), heads * dim
+    else:
+        op, os_ = _rows(out, dev, dtype, "out", (rows, heads, dim))
     tp = _table(table, i32, dev, "table")
     seqs, pages = table.shape
     L = _lib.lib()
-    need = L.yue2_attention_tree_workspace(rows, heads, seqs, pages, pool._ref)
+    need = pool._workspace(rows, heads, seqs, pages)
     work = q.new_empty((need + 1) // 2) if need else None  # 16-bit values
     _call(dev, L.yue2_attention_tree, qp, rows, heads, qs, pool._ref, layer, tp, seqs, pages,
           _flat(context, i32, dev, "context", seqs), _flat(cu, i32, dev, "cu", seqs + 1),
