@@ -104,21 +104,21 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i:
 
 
 def _flat(t, dtype, index, what, count):
-    """The address of a contiguous [count] device tensor."""
-    if t.dtype is dtype and t.get_device() == index and t.dim() == 1 and t.shape[0] == count and t.is_contiguous():
+    """The address of a contiguous device tensor of `count` values."""
+    if t.dtype is dtype and t.get_device() == index and t.numel() == count and t.is_contiguous():
         return t.data_ptr()
-    raise _invalid(f"{what} must be a contiguous [{count}] tensor of {dtype} on cuda:{index}")
+    raise _invalid(f"{what} must be a contiguous tensor of {count} {dtype} values on cuda:{index}")
 
 
 def _table(t, dtype, index, what):
-    """The address of a contiguous [rows, columns] device tensor."""
+    """The address, rows and columns of a contiguous two-dimensional device tensor."""
     if t.dtype is dtype and t.get_device() == index and t.dim() == 2 and t.is_contiguous():
-        return t.data_ptr()
+        return t.data_ptr(), *t.shape
     raise _invalid(f"{what} must be a contiguous two-dimensional tensor of {dtype} on cuda:{index}")
 
 
 def _rows(t, index, dtype, what, shape=None):
-    """The address and row stride of a [rows, heads, dim] tensor with adjacent heads."""
+    """The address, row stride and shape of a [rows, heads, dim] tensor with adjacent heads."""
     if t.dtype is not dtype or t.get_device() != index or t.dim() != 3 or (shape is not None and t.shape != shape):
         raise _invalid(f"{what} must be a [rows, heads, dim] tensor of {dtype} on cuda:{index}"
                        + (f" of shape {tuple(shape)}" if shape is not None else ""))
@@ -126,19 +126,29 @@ def _rows(t, index, dtype, what, shape=None):
     step, head, one = t.stride()
     if (one != 1 or (heads > 1 and head != dim)) and rows and heads and dim:
         raise _invalid(f"{what}: the heads of a row must be adjacent")
-    return t.data_ptr(), step if rows > 1 else heads * dim
+    return t.data_ptr(), step if rows > 1 else heads * dim, rows, heads, dim
 
 
-def _call(index, fn, *args):
-    """fn(*args, status, stream) on the device's current stream."""
-    status = _status_of(index)
-    if torch.cuda.current_device() != index:
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+def _call(index, name, *args):
+    """The library's `name`(*args, status, stream) on the device's current stream."""
+    fn = _fns.get(name)
+    if fn is None:
+        fn = _fns[name] = getattr(_lib.lib(), name)
+    s = _status.get(index)
+    status = _status_of(index) if s is None else s[0]
+    if _current_device() != index:
         with torch.cuda.device(index):
             rc = fn(*args, status, _raw_stream(index))
     else:
         rc = fn(*args, status, _raw_stream(index))
     if rc:
         _lib.check(rc)
+
+
+_fns = {}
 
 
 def qk_rope_append(qkv, q_norm, k_norm, eps, cos, sin, positions, pool, layer, slots, q_out=None, k_out=None):
@@ -149,13 +159,13 @@ def qk_rope_append(qkv, q_norm, k_norm, eps, cos, sin, positions, pool, layer, s
     slots [rows] int64, 64 * page + place, negative for a row whose K/V is not kept. Returns
     q [rows, heads, dim] (q_out when given); k_out [rows, kv, dim], when given, gets the rotated
     K as well. q_out and k_out may be the q and k parts of qkv."""
-    dev, dtype, kv = pool.index, pool.dtype, pool.kv_heads
-    src, stride = _rows(qkv, dev, dtype, "qkv")
-    rows, width, dim = qkv.shape
+    dev, dtype, kv, f32 = pool.index, pool.dtype, pool.kv_heads, torch.float32
+    src, stride, rows, width, dim = _rows(qkv, dev, dtype, "qkv")
     heads = width - 2 * kv
     if heads < 1 or dim != pool.dim:
         raise _invalid("qkv must be [rows, heads + 2 kv heads, dim] of the pool's kv heads and dim")
-    if cos.shape != sin.shape or cos.dim() != 2 or cos.shape[1] != dim // 2:
+    cp, steps, half = _table(cos, f32, dev, "cos")
+    if half != dim // 2:
         raise _invalid("cos and sin must be [table rows, dim / 2]")
     if (q_norm is None) != (k_norm is None):
         raise _invalid("q_norm and k_norm go together")
@@ -163,14 +173,13 @@ def qk_rope_append(qkv, q_norm, k_norm, eps, cos, sin, positions, pool, layer, s
         q_out = qkv.new_empty((rows, heads, dim))
         qp, qs = q_out.data_ptr(), heads * dim
     else:
-        qp, qs = _rows(q_out, dev, dtype, "q_out", (rows, heads, dim))
-    kp, ks = (0, 0) if k_out is None else _rows(k_out, dev, dtype, "k_out", (rows, kv, dim))
-    f32 = torch.float32
-    _call(dev, _lib.lib().yue2_qk_rope_append, src, rows, heads, stride,
+        qp, qs = _rows(q_out, dev, dtype, "q_out", (rows, heads, dim))[:2]
+    kp, ks = (0, 0) if k_out is None else _rows(k_out, dev, dtype, "k_out", (rows, kv, dim))[:2]
+    _call(dev, "yue2_qk_rope_append", src, rows, heads, stride,
           0 if q_norm is None else _flat(q_norm, f32, dev, "q_norm", dim),
-          0 if k_norm is None else _flat(k_norm, f32, dev, "k_norm", dim), eps, _table(cos, f32, dev, "cos"),
-          _table(sin, f32, dev, "sin"), cos.shape[0], _flat(positions, torch.int32, dev, "positions", rows), pool._ref, layer,
-          _flat(slots, torch.int64, dev, "slots", rows), qp, qs, kp if rows else 0, ks)
+          0 if k_norm is None else _flat(k_norm, f32, dev, "k_norm", dim), eps, cp, _flat(sin, f32, dev, "sin", steps * half), steps,
+          _flat(positions, torch.int32, dev, "positions", rows), pool._ref, layer, _flat(slots, torch.int64, dev, "slots", rows),
+          qp, qs, kp if rows else 0, ks)
     return q_out
 
 
@@ -185,22 +194,20 @@ def attention_packed(q, k, v, cu, causal=True, scale=None, out=None):
     code = _DTYPES.get(dtype)
     if code is None or dev < 0:
         raise _invalid("attention takes bf16 or f16 tensors on a GPU")
-    qp, qs = _rows(q, dev, dtype, "q")
-    kp, ks = _rows(k, dev, dtype, "k")
-    tokens, heads, dim = q.shape
-    kv = k.shape[1]
-    vp, vs = _rows(v, dev, dtype, "v", (tokens, kv, dim))
-    if k.shape[0] != tokens or k.shape[2] != dim:
+    qp, qs, tokens, heads, dim = _rows(q, dev, dtype, "q")
+    kp, ks, keys, kv, kdim = _rows(k, dev, dtype, "k")
+    vp, vs = _rows(v, dev, dtype, "v", (tokens, kv, dim))[:2]
+    if keys != tokens or kdim != dim:
         raise _invalid("k and v must be [tokens, kv heads, dim] of q's tokens and dim")
     if out is None:
         out = q.new_empty((tokens, heads, dim))
         op, os_ = out.data_ptr(), heads * dim
     else:
-        op, os_ = _rows(out, dev, dtype, "out", (tokens, heads, dim))
+        op, os_ = _rows(out, dev, dtype, "out", (tokens, heads, dim))[:2]
     if cu.dim() != 1 or cu.shape[0] < 1:
         raise _invalid("cu must be [seqs + 1]")
     seqs = cu.shape[0] - 1
-    _call(dev, _lib.lib().yue2_attention_packed, qp, kp, vp, op, _flat(cu, torch.int32, dev, "cu", seqs + 1), seqs, tokens,
+    _call(dev, "yue2_attention_packed", qp, kp, vp, op, _flat(cu, torch.int32, dev, "cu", seqs + 1), seqs, tokens,
           heads, kv, dim, qs, ks, vs, os_, code, 1 if causal else 0, dim ** -0.5 if scale is None else scale)
     return out
 
@@ -214,21 +221,18 @@ def attention_tree(q, pool, layer, table, context, cu, mask=None, scale=None, ou
     sequence is an ordinary decode step. A row that sees nothing gets zeros; rows outside
     [cu[0], cu[-1]) of `out` are left as they were (undefined when `out` is None)."""
     dev, dtype, i32 = pool.index, pool.dtype, torch.int32
-    qp, qs = _rows(q, dev, dtype, "q")
-    rows, heads, dim = q.shape
+    qp, qs, rows, heads, dim = _rows(q, dev, dtype, "q")
     if dim != pool.dim:
         raise _invalid("q must have the pool's dim")
     if out is None:
         out = q.new_empty((rows, heads, dim))
         op, os_ = out.data_ptr(), heads * dim
     else:
-        op, os_ = _rows(out, dev, dtype, "out", (rows, heads, dim))
-    tp = _table(table, i32, dev, "table")
-    seqs, pages = table.shape
-    L = _lib.lib()
+        op, os_ = _rows(out, dev, dtype, "out", (rows, heads, dim))[:2]
+    tp, seqs, pages = _table(table, i32, dev, "table")
     need = pool._workspace(rows, heads, seqs, pages)
     work = q.new_empty((need + 1) // 2) if need else None  # 16-bit values
-    _call(dev, L.yue2_attention_tree, qp, rows, heads, qs, pool._ref, layer, tp, seqs, pages,
+    _call(dev, "yue2_attention_tree", qp, rows, heads, qs, pool._ref, layer, tp, seqs, pages,
           _flat(context, i32, dev, "context", seqs), _flat(cu, i32, dev, "cu", seqs + 1),
           0 if mask is None else _flat(mask, torch.int64, dev, "mask", rows), dim ** -0.5 if scale is None else scale,
           op, os_, work.data_ptr() if need else 0, need)
@@ -239,7 +243,7 @@ def kv_copy(pool, src, dst, count=None):
     """Positions [0, count[i]) (all 64 when count is None) of page src[i] to page dst[i], in
     every layer; int32 [n] each. The dst pages are distinct and none of them is a src page."""
     dev, i32, n = pool.index, torch.int32, src.shape[0]
-    _call(dev, _lib.lib().yue2_kv_copy, pool._ref, _flat(src, i32, dev, "src", n), _flat(dst, i32, dev, "dst", n),
+    _call(dev, "yue2_kv_copy", pool._ref, _flat(src, i32, dev, "src", n), _flat(dst, i32, dev, "dst", n),
           0 if count is None else _flat(count, i32, dev, "count", n), n)
 
 
@@ -251,15 +255,12 @@ def kv_gather(pool, src_table, dst_table, begin, cu, keep):
     own. Otherwise into the pages of dst_table, none of which the call reads; keep in any
     order. Tables int32 [seqs, pages], begin int32 [seqs], cu int32 [seqs + 1], keep int32."""
     dev, i32 = pool.index, torch.int32
-    sp = _table(src_table, i32, dev, "src_table")
-    seqs, pages = src_table.shape
-    dp, dst_pages = 0, 0
-    if dst_table is not None:
-        dp, dst_pages = _table(dst_table, i32, dev, "dst_table"), dst_table.shape[1]
-        if dst_table.shape[0] != seqs:
-            raise _invalid("src_table and dst_table must hold the same sequences")
+    sp, seqs, pages = _table(src_table, i32, dev, "src_table")
+    dp, dst_seqs, dst_pages = (0, seqs, 0) if dst_table is None else _table(dst_table, i32, dev, "dst_table")
+    if dst_seqs != seqs:
+        raise _invalid("src_table and dst_table must hold the same sequences")
     if keep.dim() != 1:
         raise _invalid("keep must be one list")
     total = keep.shape[0]
-    _call(dev, _lib.lib().yue2_kv_gather, pool._ref, sp, pages, dp, dst_pages, _flat(begin, i32, dev, "begin", seqs),
+    _call(dev, "yue2_kv_gather", pool._ref, sp, pages, dp, dst_pages, _flat(begin, i32, dev, "begin", seqs),
           _flat(cu, i32, dev, "cu", seqs + 1), _flat(keep, i32, dev, "keep", total), seqs, total)
