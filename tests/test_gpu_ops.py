@@ -182,6 +182,59 @@ def test_packed_nonfinite_keys_are_masked(ops, value):
     assert torch.isnan(got[at]).all()  # inf - inf or NaN in its own score
 
 
+@pytest.mark.parametrize("value", [float("inf"), float("nan")])
+@pytest.mark.parametrize("at", [0, 6, 7, 13, 14, 15, 31, 64, 127, 128, 255, 511])
+def test_packed_nonfinite_scores_make_their_rows_nan(ops, at, value):
+    # in tiles that every row sees and in the last, at places of either way of exponentials
+    n = 700
+    q, k, v = randn((n, 1, 128), torch.bfloat16, 1), randn((n, 1, 128), torch.bfloat16, 2), randn((n, 1, 128), torch.bfloat16, 3)
+    clean = ops.attention_packed(q, k, v, offsets([n]))
+    k[at] = value
+    got = ops.attention_packed(q, k, v, offsets([n]))
+    assert torch.equal(got[:at], clean[:at])
+    assert torch.isnan(got[at:]).all()
+
+
+@pytest.mark.parametrize("dtype,huge", [(torch.bfloat16, 3.0e38), (torch.float16, 65504.0)])
+def test_packed_huge_values_in_masked_places(ops, dtype, huge):
+    q, k, v = randn((500, 2, 64), dtype, 1), randn((500, 1, 64), dtype, 2), randn((500, 1, 64), dtype, 3)
+    clean = ops.attention_packed(q, k, v, offsets([300, 150]))[:450].clone()
+    v[100:300] = huge
+    k[100:300] = huge / 2 if dtype == torch.bfloat16 else 100.0
+    v[450:], k[450:] = -huge, huge
+    got = ops.attention_packed(q, k, v, offsets([300, 150]))
+    assert torch.equal(got[:100], clean[:100]) and torch.equal(got[300:450], clean[300:450])
+
+
+def test_packed_at_the_limits(ops):
+    rng = random.Random(8)
+    lens = [rng.choice([0, 1, 2, 3, 7]) for _ in range(1024)]
+    check_packed(ops, lens, 1, 1, 64, torch.bfloat16, True, behind=2)
+    # 262,144 tokens, most of them behind the last sequence
+    n = 1 << 18
+    q = randn((n, 1, 64), torch.bfloat16, 1)
+    lens = [500, 0, 77]
+    out = torch.full_like(q, 2.0)
+    ops.attention_packed(q, q, q, offsets(lens, n - 600), out=out)
+    want, tol = packed_reference(q[n - 600:], q[n - 600:], q[n - 600:], lens, 0, True, 1 / 8)
+    close(out[n - 600:n - 23], want[:577], tol[:577])
+    assert (out[:n - 600] == 2).all() and (out[n - 23:] == 2).all()
+    big = torch.empty((n + 1, 1, 64), dtype=torch.bfloat16, device=DEV)
+    with pytest.raises(Yue2Error, match="262,144"):
+        ops.attention_packed(big, big, big, offsets([5]))
+    with pytest.raises(Yue2Error, match="1,024"):
+        ops.attention_packed(q, q, q, offsets([1] * 1025))
+
+
+def test_packed_output_over_its_queries(ops):
+    # every unit has its queries before it writes, and no other reads them
+    qkv = randn((700, 8, 128), torch.bfloat16, 1)
+    q, k, v = qkv[:, :4], qkv[:, 4:6], qkv[:, 6:]
+    want = ops.attention_packed(q, k, v, offsets([400, 300]))
+    ops.attention_packed(q, k, v, offsets([400, 300]), out=q)
+    assert torch.equal(q, want)
+
+
 def test_packed_repeats_bit_for_bit_and_on_another_stream(ops):
     q, k, v = randn((900, 8, 128), torch.bfloat16, 1), randn((900, 2, 128), torch.bfloat16, 2), randn((900, 2, 128), torch.bfloat16, 3)
     cu = offsets([300, 1, 599])
@@ -313,7 +366,8 @@ def test_tree_lengths(ops, ctx, nodes, masks):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
-@pytest.mark.parametrize("heads,kv,dim", [(24, 8, 128), (8, 2, 128), (4, 2, 64), (2, 2, 64), (8, 1, 128), (16, 1, 64), (5, 1, 64)])
+@pytest.mark.parametrize("heads,kv,dim", [(24, 8, 128), (8, 2, 128), (4, 2, 64), (2, 2, 64), (8, 1, 128), (16, 1, 64), (5, 1, 64),
+                                          (96, 1, 128), (128, 1, 64)])
 def test_tree_layouts(ops, heads, kv, dim, dtype):
     check_tree(ops, [130, 0, 700, 64, 5], [9, 3, 1, 0, 33], heads, kv, dim, dtype, first=2, behind=3)
     check_tree(ops, [77, 2000], [64, 1], heads, kv, dim, dtype, None, layers=1, layer=0)
@@ -368,6 +422,55 @@ def test_tree_nonfinite_drafts_stay_with_the_rows_that_see_them(ops, value):
     assert torch.equal(got[~sees], clean[~sees])
     hit = got[sees]
     assert torch.isnan(hit).all() if math.isnan(value) else (hit == value).all()
+
+
+@pytest.mark.parametrize("value", [float("inf"), float("nan")])
+@pytest.mark.parametrize("at", [0, 7, 14, 15, 127, 128, 299, 300, 305])
+def test_tree_nonfinite_scores_make_their_rows_nan(ops, at, value):
+    ctx, nodes = 300, 12
+    rng = random.Random(2)
+    pages, table = make_pages(rng, [ctx + nodes])
+    data = randn((pages, 1, 2, 1, 64, 64), torch.bfloat16, 4)
+    q = randn((nodes, 3, 64), torch.bfloat16, 5)
+    mask = tree_masks(rng, [nodes])
+    args = (q, ops.KvPool(data), 0, ints(table), ints([ctx]), offsets([nodes]), ints(mask.view(np.int64), torch.int64))
+    clean = ops.attention_tree(*args)
+    data[table[0, at // 64], 0, 0, 0, at % 64] = value
+    got = ops.attention_tree(*args)
+    for i in range(nodes):
+        if at < ctx or int(mask[i]) >> (at - ctx) & 1:
+            assert torch.isnan(got[i]).all()
+        else:
+            assert torch.equal(got[i], clean[i])
+
+
+def test_tree_huge_values_in_masked_places(ops):
+    rng = random.Random(2)
+    ctx, nodes = 60, 40
+    pages, table = make_pages(rng, [ctx + nodes])
+    data = randn((pages, 1, 2, 1, 64, 128), torch.bfloat16, 4)
+    q = randn((nodes, 4, 128), torch.bfloat16, 5)
+    args = (q, ops.KvPool(data), 0, ints(table), ints([ctx]), offsets([nodes]))
+    clean = ops.attention_tree(*args)
+    for p in range(ctx + 20, ctx + nodes):
+        data[table[0, p // 64], 0, :, 0, p % 64] = 3.0e38
+    got = ops.attention_tree(*args)
+    assert torch.equal(got[:20], clean[:20])
+
+
+def test_tree_at_the_limits(ops):
+    rng = random.Random(9)
+    n = 1024
+    check_tree(ops, [rng.choice([0, 1, 63, 64, 70]) for _ in range(n)], [rng.choice([0, 1, 1, 2]) for _ in range(n)], 2, 1, 64, torch.bfloat16, None,
+               layers=1, layer=0)
+    check_tree(ops, [0] * 20, [64] * 20, 8, 1, 64, torch.float16, layers=1, layer=0)
+    pool = ops.KvPool(randn((2, 1, 2, 1, 64, 64), torch.bfloat16, 1))
+    q = randn((1025, 1, 64), torch.bfloat16, 2)
+    with pytest.raises(Yue2Error, match="1,024"):
+        ops.attention_tree(q, pool, 0, ints([[0]] * 1025), ints([0] * 1025), offsets([1] * 1025))
+    wide = ops.KvPool(randn((2, 1, 2, 1, 64, 64), torch.bfloat16, 1))
+    with pytest.raises(Yue2Error, match="128 query heads"):
+        ops.attention_tree(randn((1, 129, 64), torch.bfloat16, 2), wide, 0, ints([[0]]), ints([0]), offsets([1]))
 
 
 def test_tree_shared_pages_and_strided_rows(ops):
@@ -698,6 +801,21 @@ def test_a_step_over_a_batch(ops, heads, kv, dim, dtype):
             g = h // (heads // kv)
             want, tol = attend(q[s:s + 1, h], kk[:, g], vv[:, g], see, 1 / math.sqrt(dim))
             close(got[s:s + 1, h], want, tol, (s, h))
+
+
+def test_first_call_inside_a_capture_is_refused(ops, monkeypatch):
+    # the status word would belong to the graph
+    data = randn((2, 1, 2, 1, 64, 64), torch.bfloat16, 1)
+    pool = ops.KvPool(data)
+    src, dst = ints([0]), ints([1])
+    monkeypatch.setattr(ops, "_status", {})
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(Yue2Error, match="before any capture"):
+        ops.kv_copy(pool, src, dst)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    ops.kv_copy(pool, src, dst)
+    ops.check_status()
+    assert torch.equal(data[0], data[1])
 
 
 def test_python_refusals(ops):
