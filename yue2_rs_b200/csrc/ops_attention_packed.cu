@@ -230,7 +230,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         auto part = [&] { announce(p_part); };
         if (masked || a.negate) softmax_tile<D, F16, false>(s_addr, o_addr, a.c, a.negate, j == 0, vis, st, part);
-        else softmax_tile<D, F16, true>(s_addr, o_addr, a.c, false, j == 0, vis, st, part);
+        else if (j == 0 || !softmax_settled<D, F16>(s_addr, a.c, st, part))
+          softmax_tile<D, F16, true>(s_addr, o_addr, a.c, false, j == 0, vis, st, part);
         announce(p_full);
       }
       if (!ok) break;

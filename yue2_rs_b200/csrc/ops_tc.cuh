@@ -253,7 +253,7 @@ Y2_DEV void take_scores(uint32_t (&v)[32], bool negate, uint32_t vis) {
 // the output's own rounding; l sums the unrounded weights). With PLAIN, kPoly of 16 pairs take the FMA
 // units, the others the special-function unit, which alone would need as long as the tensor
 // cores (8,192 rows of 24 heads: 787 us with 0, 764 with 2, 762 with 4, 759 with 8; masked keys need exact zeros). part() runs when 96 weights are stored; the caller announces the last 32.
-constexpr int kPoly = 4;
+constexpr int kPoly = 2;
 template <int D, bool F16, bool PLAIN, class Part>
 Y2_DEV void softmax_tile(uint32_t s_addr, uint32_t o_addr, float c, bool negate, bool first, const uint32_t (&vis)[4],
                          RowStats& st, Part part) {
@@ -326,6 +326,63 @@ Y2_DEV void softmax_tile(uint32_t s_addr, uint32_t o_addr, float c, bool negate,
     store16(s_addr + 16 * q, p);
     if (q == 2) part();
   }
+}
+
+// The same for a tile that every row sees whole, with a positive scale, after the first one: the
+// weights are formed relative to the m there is, the maximum is found on the way, and only
+// when it asks for another m (false: nothing has been written) softmax_tile does the tile. Without the
+// first pass the exponentials start as soon as the scores are there.
+template <int D, bool F16, class Part>
+Y2_DEV bool softmax_settled(uint32_t s_addr, float c, RowStats& st, Part part) {
+  const float mc = st.m == -INFINITY ? 0.f : st.m == INFINITY ? NAN : -st.m * c;
+  uint32_t v[2][32], p[3][16];
+  float l[4] = {0.f, 0.f, 0.f, 0.f}, mx = -INFINITY, my = -INFINITY;
+  auto weights = [&](float a, float b, int i, float (&sum)[4]) {
+    if (i % (16 / kPoly) == 16 / kPoly - 1) {
+      poly_ex2<F16>(a, b);
+    } else {
+      a = ex2(a);
+      b = ex2(b);
+    }
+    add2(sum[2 * (i & 1)], sum[2 * (i & 1) + 1], a, b);
+    return pack16<F16>(a, b);
+  };
+  load32(s_addr, v[0]);
+#pragma unroll
+  for (int q = 0; q < 3; ++q) {
+    uint32_t(&s)[32] = v[q & 1];
+    wait_loads();
+    arrived(s);
+    load32(s_addr + 32 * (q + 1), v[(q + 1) & 1]);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      float a, b;
+      fma2(a, b, __uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]), c, c, mc, mc);
+      if (i & 1) mx = max3(mx, a, b);
+      else my = max3(my, a, b);
+      p[q][i] = weights(a, b, i, l);
+    }
+  }
+  uint32_t(&s)[32] = v[1];
+  float x[32];
+  wait_loads();
+  arrived(s);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    fma2(x[2 * i], x[2 * i + 1], __uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]), c, c, mc, mc);
+    if (i & 1) mx = max3(mx, x[2 * i], x[2 * i + 1]);
+    else my = max3(my, x[2 * i], x[2 * i + 1]);
+  }
+  if (__any_sync(0xffffffffu, !(max3(mx, my, my) <= 8.0f))) return false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) st.l[i] += l[i];
+#pragma unroll
+  for (int q = 0; q < 3; ++q) store16(s_addr + 16 * q, p[q]);
+  part();
+#pragma unroll
+  for (int i = 0; i < 16; ++i) p[0][i] = weights(x[2 * i], x[2 * i + 1], i, st.l);
+  store16(s_addr + 48, p[0]);
+  return true;
 }
 
 // Key `r` of a V tile in shared memory (slabs of [128][64 dims], 128-byte swizzle), 64 dims of
