@@ -229,9 +229,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           tc::fence_proxy_async();
         }
         auto part = [&] { announce(p_part); };
-        if (masked || a.negate) softmax_tile<D, F16, false>(s_addr, o_addr, a.c, a.negate, j == 0, vis, st, part);
+        if (masked || a.negate) softmax_masked<D, F16, 4>(s_addr, o_addr, a.c, a.negate, j == 0, vis, st, part);
         else if (j == 0 || !softmax_settled<D, F16>(s_addr, a.c, st, part))
-          softmax_tile<D, F16, true>(s_addr, o_addr, a.c, false, j == 0, vis, st, part);
+          softmax_tile<D, F16>(s_addr, o_addr, a.c, j == 0, st, part);
         announce(p_full);
       }
       if (!ok) break;

@@ -233,10 +233,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           uint32_t vis[4];
 #pragma unroll
           for (int q = 0; q < 4; ++q) vis[q] = seen_bits(key0 + 32 * q, u.ctx, mask);
-          softmax_tile<D, F16, false>(s_addr, o_addr, a.c, a.negate, i == 0, vis, st, part);
+          softmax_masked<D, F16, 1>(s_addr, o_addr, a.c, a.negate, i == 0, vis, st, part);
         } else {
-          const uint32_t vis[4] = {};
-          softmax_tile<D, F16, true>(s_addr, o_addr, a.c, false, i == 0, vis, st, part);
+          softmax_tile<D, F16>(s_addr, o_addr, a.c, i == 0, st, part);
         }
         announce(p_full);
       }

@@ -220,65 +220,13 @@ Y2_DEV void poly_ex2(float& x, float& y) {
   y = __uint_as_float(__float_as_uint(py) + (__float_as_uint(ny) << 23));
 }
 
-// 32 scores with the sign of the scale and without the keys that the row does not see. PLAIN:
-// a positive scale and every key seen. (Branches around the plain form would cut the code
-// into blocks across which loads, exponentials and products no longer overlap.)
-template <bool PLAIN>
-Y2_DEV void take_scores(uint32_t (&v)[32], bool negate, uint32_t vis) {
-  if constexpr (!PLAIN) {
-    if (negate) {
-#pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] ^= 0x80000000u;
-    }
-    if (!__all_sync(0xffffffffu, vis == 0xffffffffu)) {
-#pragma unroll
-      for (int i = 0; i < 32; ++i)
-        if (!(vis >> i & 1)) v[i] = 0xff800000u;
-    }
-  }
-}
-
-// A side's softmax over one tile of 128 keys: the scores in TMEM become weights
-// p = 2^(c (s - m)), packed over them. c = |scale| log2(e), `negate` for a negative scale; bit i of
-// `vis` says whether the row sees key i (both only without PLAIN). Every lane of the warp takes part.
-//
-// The maximum first. m starts as the first tile's and moves, O and l being scaled by
-// 2^(c (m_old - m_new)), only when a score exceeds it by more than a factor 2^8 of weight:
-// until then the weights are at most 2^8, exact in the f32 sums, and the final division by l
-// removes the factor. So most tiles leave O alone. O is settled: the P.V of the previous tile
-// was issued before the scores of this one. A score of +inf or NaN makes m so and the row NaN.
-//
-// Then the weights, in a second pass over the scores in TMEM (reading them again costs less
-// than holding 128 registers). p is rounded to 16 bits (relative error of half a step, as
-// the output's own rounding; l sums the unrounded weights). With PLAIN, kPoly of 16 pairs take the FMA
-// units, the others the special-function unit, which alone would need as long as the tensor
-// cores (8,192 rows of 24 heads: 787 us with 0, 764 with 2, 762 with 4, 759 with 8; masked keys need exact zeros). part() runs when 96 weights are stored; the caller announces the last 32.
-constexpr int kPoly = 2;
-template <int D, bool F16, bool PLAIN, class Part>
-Y2_DEV void softmax_tile(uint32_t s_addr, uint32_t o_addr, float c, bool negate, bool first, const uint32_t (&vis)[4],
-                         RowStats& st, Part part) {
-  uint32_t v[2][32];
-  float mx[4] = {st.m, st.m, st.m, st.m};
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    load32(s_addr + 64 * h, v[0]);
-    load32(s_addr + 64 * h + 32, v[1]);
-    wait_loads();
-    arrived(v[0]);
-    arrived(v[1]);
-    take_scores<PLAIN>(v[0], negate, vis[2 * h]);
-    take_scores<PLAIN>(v[1], negate, vis[2 * h + 1]);
-#pragma unroll
-    for (int i = 0; i < 32; i += 4) {
-      mx[0] = max3(mx[0], __uint_as_float(v[0][i]), __uint_as_float(v[0][i + 1]));
-      mx[1] = max3(mx[1], __uint_as_float(v[0][i + 2]), __uint_as_float(v[0][i + 3]));
-      mx[2] = max3(mx[2], __uint_as_float(v[1][i]), __uint_as_float(v[1][i + 1]));
-      mx[3] = max3(mx[3], __uint_as_float(v[1][i + 2]), __uint_as_float(v[1][i + 3]));
-    }
-  }
-  load32(s_addr, v[0]);
-  const float mn = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]);
-  // NaN moves too; a row that has seen nothing yet stays
+// A new maximum mn of a row (NaN moves m too; a row that has seen nothing yet stays): m moves, and O
+// and l are scaled by 2^(c (m_old - m_new)), only when a score exceeds m by more than a factor
+// 2^8 of weight: until then the weights are at most 2^8, exact in the f32 sums, and the final
+// division by l removes the factor. So most tiles leave O alone. O is settled: the P.V of the
+// previous tile was issued before the scores of this one.
+template <int D>
+Y2_DEV void move_max(uint32_t o_addr, float c, bool first, float mn, RowStats& st) {
   const bool move = first || (mn != -INFINITY && !((mn - st.m) * c <= 8.0f));
   if (!first && __any_sync(0xffffffffu, move)) {
     const float alpha = move ? ex2((st.m - mn) * c) : 1.0f;
@@ -294,7 +242,43 @@ Y2_DEV void softmax_tile(uint32_t s_addr, uint32_t o_addr, float c, bool negate,
     }
   }
   if (move) st.m = mn;
-  const float mc = st.m == -INFINITY ? 0.f : st.m == INFINITY ? NAN : -st.m * c;
+}
+// -c m, the constant of the exponent. A score of +inf or NaN makes m so and the row NaN.
+Y2_DEV float exponent_base(float c, const RowStats& st) {
+  return st.m == -INFINITY ? 0.f : st.m == INFINITY ? NAN : -st.m * c;
+}
+
+// A side's softmax over one tile of 128 keys: the scores in TMEM become weights
+// p = 2^(c (s - m)), packed over them. c = |scale| log2(e). Every lane of the warp takes part.
+// The maximum first (m starts as the first tile's), then the weights in a second pass over the
+// scores in TMEM (reading them again costs less than holding 128 registers). p is rounded
+// to 16 bits (relative error of half a step, as the output's own rounding; l sums the
+// unrounded weights). kPoly of 16 pairs take the FMA units, the others the special-function
+// unit, which alone would need as long as the tensor cores. part() runs when 96 weights are
+// stored; the caller announces the last 32.
+constexpr int kPoly = 2;
+template <int D, bool F16, class Part>
+Y2_DEV void softmax_tile(uint32_t s_addr, uint32_t o_addr, float c, bool first, RowStats& st, Part part) {
+  uint32_t v[2][32];
+  float mx[4] = {st.m, st.m, st.m, st.m};
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    load32(s_addr + 64 * h, v[0]);
+    load32(s_addr + 64 * h + 32, v[1]);
+    wait_loads();
+    arrived(v[0]);
+    arrived(v[1]);
+#pragma unroll
+    for (int i = 0; i < 32; i += 4) {
+      mx[0] = max3(mx[0], __uint_as_float(v[0][i]), __uint_as_float(v[0][i + 1]));
+      mx[1] = max3(mx[1], __uint_as_float(v[0][i + 2]), __uint_as_float(v[0][i + 3]));
+      mx[2] = max3(mx[2], __uint_as_float(v[1][i]), __uint_as_float(v[1][i + 1]));
+      mx[3] = max3(mx[3], __uint_as_float(v[1][i + 2]), __uint_as_float(v[1][i + 3]));
+    }
+  }
+  load32(s_addr, v[0]);
+  move_max<D>(o_addr, c, first, max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]), st);
+  const float mc = exponent_base(c, st);
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     uint32_t(&s)[32] = v[q & 1];
@@ -302,19 +286,11 @@ Y2_DEV void softmax_tile(uint32_t s_addr, uint32_t o_addr, float c, bool negate,
     arrived(s);
     if (q < 3) load32(s_addr + 32 * (q + 1), v[(q + 1) & 1]);
     uint32_t p[16];
-    if (!PLAIN && __all_sync(0xffffffffu, vis[q] == 0)) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) p[i] = 0;
-      store16(s_addr + 16 * q, p);
-      if (q == 2) part();
-      continue;
-    }
-    take_scores<PLAIN>(s, negate, vis[q]);
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       float a, b;
       fma2(a, b, __uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]), c, c, mc, mc);
-      if (PLAIN && i % (16 / kPoly) == 16 / kPoly - 1) {
+      if (i % (16 / kPoly) == 16 / kPoly - 1) {
         poly_ex2<F16>(a, b);
       } else {
         a = ex2(a);
@@ -328,13 +304,66 @@ Y2_DEV void softmax_tile(uint32_t s_addr, uint32_t o_addr, float c, bool negate,
   }
 }
 
+// The same where rows do not see every key (bit i of `vis`) or the scale is negative. Once or twice
+// a unit; UNROLL 1 keeps it small, as its instructions come from far away (tree attention:
+// full trees 65.4 -> 62.6 us; packed attention is faster with 4: two prompts 31.3 -> 30.8).
+// Masked keys need exact zeros, so no weight is a polynomial's.
+template <int D, bool F16, int UNROLL, class Part>
+Y2_DEV void softmax_masked(uint32_t s_addr, uint32_t o_addr, float c, bool negate, bool first, const uint32_t (&vis)[4],
+                           RowStats& st, Part part) {
+  const uint32_t sign = negate ? 0x80000000u : 0u;
+  uint32_t v[32];
+  auto take = [&](int q) {
+    const uint32_t bits = vis[q];
+    load32(s_addr + 32 * q, v);
+    wait_loads();
+    arrived(v);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = bits >> i & 1 ? v[i] ^ sign : 0xff800000u;
+  };
+  float mx = st.m, my = st.m;
+#pragma unroll UNROLL
+  for (int q = 0; q < 4; ++q) {
+    if (__all_sync(0xffffffffu, vis[q] == 0)) continue;
+    take(q);
+#pragma unroll
+    for (int i = 0; i < 32; i += 4) {
+      mx = max3(mx, __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+      my = max3(my, __uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]));
+    }
+  }
+  move_max<D>(o_addr, c, first, max3(mx, my, my), st);
+  const float mc = exponent_base(c, st);
+#pragma unroll UNROLL
+  for (int q = 0; q < 4; ++q) {
+    uint32_t p[16];
+    if (__all_sync(0xffffffffu, vis[q] == 0)) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) p[i] = 0;
+    } else {
+      take(q);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        float a, b;
+        fma2(a, b, __uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]), c, c, mc, mc);
+        a = ex2(a);
+        b = ex2(b);
+        add2(st.l[2 * (i & 1)], st.l[2 * (i & 1) + 1], a, b);
+        p[i] = pack16<F16>(a, b);
+      }
+    }
+    store16(s_addr + 16 * q, p);
+    if (q == 2) part();
+  }
+}
+
 // The same for a tile that every row sees whole, with a positive scale, after the first one: the
 // weights are formed relative to the m there is, the maximum is found on the way, and only
 // when it asks for another m (false: nothing has been written) softmax_tile does the tile. Without the
 // first pass the exponentials start as soon as the scores are there.
 template <int D, bool F16, class Part>
 Y2_DEV bool softmax_settled(uint32_t s_addr, float c, RowStats& st, Part part) {
-  const float mc = st.m == -INFINITY ? 0.f : st.m == INFINITY ? NAN : -st.m * c;
+  const float mc = exponent_base(c, st);
   uint32_t v[2][32], p[3][16];
   float l[4] = {0.f, 0.f, 0.f, 0.f}, mx = -INFINITY, my = -INFINITY;
   auto weights = [&](float a, float b, int i, float (&sum)[4]) {
