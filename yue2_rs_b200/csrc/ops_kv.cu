@@ -144,7 +144,8 @@ void launch_append(const AppendParams& p, unsigned rows, cudaStream_t st) {
 }
 
 // ------------------------------------------------------------------ page copy
-// CTA (block b, pair i): the first count[i] positions of one [64][dim] block, 16 KB at most.
+// CTA (block b, pair i): the first count[i] positions of one [64][dim] block, 32 KB at most,
+// four 16-byte words of a thread in flight.
 constexpr int kMoveThreads = 256;
 
 __global__ void __launch_bounds__(kMoveThreads) kv_copy_kernel(PoolView pool, const int32_t* src, const int32_t* dst,
@@ -161,7 +162,15 @@ __global__ void __launch_bounds__(kMoveThreads) kv_copy_kernel(PoolView pool, co
   const uint4* from = reinterpret_cast<const uint4*>(pool.base + a * pool.page_stride + block);
   uint4* to = reinterpret_cast<uint4*>(pool.base + b * pool.page_stride + block);
   const int words = n * pool.dim / 8;
-  for (int w = threadIdx.x; w < words; w += kMoveThreads) to[w] = from[w];
+  for (int w0 = threadIdx.x; w0 < words; w0 += 4 * kMoveThreads) {
+    uint4 v[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (w0 + u * kMoveThreads < words) v[u] = from[w0 + u * kMoveThreads];
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (w0 + u * kMoveThreads < words) to[w0 + u * kMoveThreads] = v[u];
+  }
 }
 
 // ------------------------------------------------------------------ position moves
