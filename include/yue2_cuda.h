@@ -361,8 +361,8 @@ int yue2_bench_gemv(Yue2Model* m, int kind, int rows, int launches, double* avg_
  * replay may change their contents. Calls on different streams may overlap as long as their
  * outputs and workspaces differ. The host checks sizes, strides, types and alignment and
  * returns YUE2_ERR_INVALID before any launch. What only the device sees (page indexes,
- * lengths, positions) is checked there: an entry out of range is skipped, so nothing outside
- * the buffers is touched, and a YUE2_STATUS_* bit is set (atomic or) in `status`, one int32
+ * lengths, positions) is checked there: nothing outside the buffers is touched for an entry out
+ * of range, and a YUE2_STATUS_* bit is set (atomic or) in `status`, one int32
  * that the caller clears and reads when it likes.
  *
  * Vectors of one head are contiguous and the heads of a row adjacent; row strides are in
@@ -387,7 +387,8 @@ typedef struct {
  * qkv [rows, heads + 2 kv, dim]. f32 throughout, one rounding. slots[row] < 0 writes no K/V;
  * distinct rows have distinct slots. q_out [rows, heads, dim] and, when not NULL, k_out
  * [rows, kv, dim] get the rotated heads; they may be the q and k parts of qkv itself (same
- * base and stride). A row whose position is out of range is skipped whole. */
+ * base and stride). A row whose position is out of range is skipped whole; one whose slot is
+ * outside the pool writes no K/V. cos, sin and the gains are 16-byte aligned. */
 int yue2_qk_rope_append(const void* qkv, uint64_t rows, uint64_t heads, uint64_t qkv_stride, const float* q_norm,
                         const float* k_norm, float eps, const float* cos, const float* sin, uint64_t table_rows,
                         const int32_t* positions, const Yue2KvPool* pool, uint64_t layer, const int64_t* slots,
@@ -398,8 +399,10 @@ int yue2_qk_rope_append(const void* qkv, uint64_t rows, uint64_t heads, uint64_t
  * k and v [tokens, kv, dim] are sequence s (cu: int32 [seqs + 1], nondecreasing, empty
  * sequences allowed; at most 1,024 sequences and 262,144 tokens). A row sees the rows of its
  * sequence up to itself (causal != 0) or all of them; out = softmax(scale q.k) v in `dtype`.
- * Rows outside [cu[0], cu[seqs]) are neither read nor written, and what a masked position
- * holds (infinities and NaN included) reaches no output. dim 64 or 128, heads a multiple of kv. */
+ * Rows of `out` outside [cu[0], cu[seqs]) are left as they were, and what a masked position or a
+ * row outside the sequence holds (infinities and NaN included) reaches no output. `out` may be
+ * q itself (same base and stride) and overlaps neither k nor v. dim 64 or 128, heads a
+ * multiple of kv. */
 int yue2_attention_packed(const void* q, const void* k, const void* v, void* out, const int32_t* cu, uint64_t seqs,
                           uint64_t tokens, uint64_t heads, uint64_t kv, uint64_t dim, uint64_t q_stride,
                           uint64_t k_stride, uint64_t v_stride, uint64_t out_stride, int32_t dtype, int32_t causal,
@@ -410,8 +413,11 @@ int yue2_attention_packed(const void* q, const void* k, const void* v, void* out
  * whose K/V are already in the pages (yue2_qk_rope_append). Row cu[s] + i of q [rows, heads,
  * dim] sees the whole context and the drafted positions context[s] + j whose bit j is set in
  * mask[cu[s] + i] (a node's ancestors and itself; bits >= T are ignored); mask NULL: j <= i,
- * so T = 1 is an ordinary decode step. A row that sees nothing gets zeros; rows outside
- * [cu[0], cu[seqs]) are left as they were. At most 1,024 sequences. `workspace`:
+ * so T = 1 is an ordinary decode step. A row that sees nothing gets zeros; rows of `out`
+ * outside [cu[0], cu[seqs]) are left as they were; what a masked or unused place of a page holds
+ * reaches no output; a sequence with a bad page index has undefined outputs. `out` does not
+ * overlap q. At most 1,024 sequences and 128 query heads per kv head, and a pool of fewer
+ * than 2^31 [dim] rows. `workspace`:
  * yue2_attention_tree_workspace bytes (0: may be NULL), 16-byte aligned, contents free before
  * and after; calls that may overlap need their own. */
 uint64_t yue2_attention_tree_workspace(uint64_t rows, uint64_t heads, uint64_t seqs, uint64_t table_pages,

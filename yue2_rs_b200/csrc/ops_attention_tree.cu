@@ -14,6 +14,13 @@
 // lengths on the device, so the host needs none of them.
 //
 // A CTA is ten warps as in attention_packed: softmax of the sides, products, page loads (TMA).
+//
+// Measured on one B200, captured: trees of 64 and 48 nodes over 24,512 and 20,001 positions (24 / 8
+// heads of 128) 63 us against 28 us for the bytes alone; about 6 us pass before the first
+// weights (shares, page table, first tiles), a tile then takes 1.9 us (two sides of
+// products and softmax; the bytes alone 1.5), the partial results 3 and the merge 4. A batch of eight
+// trees at 63..8,191 positions 44 us against 18; one token of two sequences at 1,030
+// positions 15 us, all of it latency.
 #include <algorithm>
 #include <atomic>
 #include <cmath>

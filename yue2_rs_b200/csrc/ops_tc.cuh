@@ -254,8 +254,9 @@ Y2_DEV float exponent_base(float c, const RowStats& st) {
 // scores in TMEM (reading them again costs less than holding 128 registers). p is rounded
 // to 16 bits (relative error of half a step, as the output's own rounding; l sums the
 // unrounded weights). kPoly of 16 pairs take the FMA units, the others the special-function
-// unit, which alone would need as long as the tensor cores. part() runs when 96 weights are
-// stored; the caller announces the last 32.
+// unit, which alone would need as long as the tensor cores (8,192 rows of 24 heads: 719 us
+// with 0, 712 with 1, 711 with 2, 729 with 4, 767 with 8, where the additional instructions cost
+// more). part() runs when 96 weights are stored; the caller announces the last 32.
 constexpr int kPoly = 2;
 template <int D, bool F16, class Part>
 Y2_DEV void softmax_tile(uint32_t s_addr, uint32_t o_addr, float c, bool first, RowStats& st, Part part) {
@@ -306,7 +307,7 @@ Y2_DEV void softmax_tile(uint32_t s_addr, uint32_t o_addr, float c, bool first, 
 
 // The same where rows do not see every key (bit i of `vis`) or the scale is negative. Once or twice
 // a unit; UNROLL 1 keeps it small, as its instructions come from far away (tree attention:
-// full trees 65.4 -> 62.6 us; packed attention is faster with 4: two prompts 31.3 -> 30.8).
+// full trees 65.4 -> 62.6 us; packed attention is as fast with 4).
 // Masked keys need exact zeros, so no weight is a polynomial's.
 template <int D, bool F16, int UNROLL, class Part>
 Y2_DEV void softmax_masked(uint32_t s_addr, uint32_t o_addr, float c, bool negate, bool first, const uint32_t (&vis)[4],
@@ -359,8 +360,10 @@ Y2_DEV void softmax_masked(uint32_t s_addr, uint32_t o_addr, float c, bool negat
 
 // The same for a tile that every row sees whole, with a positive scale, after the first one: the
 // weights are formed relative to the m there is, the maximum is found on the way, and only
-// when it asks for another m (false: nothing has been written) softmax_tile does the tile. Without the
-// first pass the exponentials start as soon as the scores are there.
+// when it asks for another m (false: nothing has been written) softmax_masked does the tile.
+// Without the first pass the exponentials start as soon as the scores are there (8,192 rows of
+// 24 heads, all seen: 756 -> 716 us). Only long packed sequences gain: in tree attention
+// the larger code costs more than the pass (full trees 65.2 -> 67.8 us).
 template <int D, bool F16, class Part>
 Y2_DEV bool softmax_settled(uint32_t s_addr, float c, RowStats& st, Part part) {
   const float mc = exponent_base(c, st);
