@@ -143,7 +143,9 @@ int ensure_scratch(DropIn& d, size_t hidden, size_t heads, size_t kv, size_t dim
       !dalloc(d, (void**)&d.cos_tab, (size_t)kContext * dim / 2 * 4) ||
       !dalloc(d, (void**)&d.sin_tab, (size_t)kContext * dim / 2 * 4))
     return 0;
-  if (!ok_or(cudaMemset(d.counters, 0, kv * 4), "memset") || !ok_or(cudaMemset(d.flags, 0, 64), "memset")) return 0;
+  if (!ok_or(cudaMemsetAsync(d.counters, 0, kv * 4, d.stream), "memset") ||
+      !ok_or(cudaMemsetAsync(d.flags, 0, 64, d.stream), "memset"))
+    return 0;
   d.cap_hidden = hidden;
   d.cap_q = q;
   d.cap_kv = kd;

@@ -547,19 +547,21 @@ int yue2_model_finalize(Yue2Model* m) {
     m->part = (float*)p;
     if ((rc = m->alloc(&p, R * g.kvh * 4))) return rc;
     m->counters = (int32_t*)p;
-    CK(cudaMemset(p, 0, R * g.kvh * 4));
+    CK(cudaMemsetAsync(p, 0, R * g.kvh * 4, m->stream));
     if ((rc = m->alloc(&p, R * sizeof(DevRow)))) return rc;
     m->rows = (DevRow*)p;
     if ((rc = m->alloc(&p, 256))) return rc;
     m->flags = (int32_t*)p;
-    CK(cudaMemset(p, 0, 256));
+    CK(cudaMemsetAsync(p, 0, 256, m->stream));
     if (m->tp_world > 1) {  // tensor-parallel exchange buffers (tp.cu)
       if ((rc = m->alloc(&p, tp_recv_bytes(g.hidden, g.vocab)))) return rc;
       m->tp_recv = (char*)p;
-      CK(cudaMemset(p, 0, tp_recv_bytes(g.hidden, g.vocab)));
+      CK(cudaMemsetAsync(p, 0, tp_recv_bytes(g.hidden, g.vocab), m->stream));
       if ((rc = m->alloc(&p, 256))) return rc;
       m->tp_epoch = (uint32_t*)p;
-      CK(cudaMemset(p, 0, 256));
+      CK(cudaMemsetAsync(p, 0, 256, m->stream));
+      // the peers write there as soon as they are connected
+      CK(cudaStreamSynchronize(m->stream));
     }
     CK(cudaMallocHost(&m->pinned_rows, Yue2Model::kRowSlots * R * sizeof(DevRow)));
     CK(cudaMallocHost(&m->pinned_flags, 4096));

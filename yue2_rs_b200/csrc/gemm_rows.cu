@@ -202,7 +202,8 @@ static int ensure_prefill(Yue2Model& m) {
     delete P;
     return rc;
   }
-  cudaError_t e = cudaMemset(P->counters, 0, (size_t)C * g.kvh * 4);
+  // on the model's stream: it does not wait for the default one
+  cudaError_t e = cudaMemsetAsync(P->counters, 0, (size_t)C * g.kvh * 4, m.stream);
 
   if (e != cudaSuccess) {
     delete P;
@@ -555,7 +556,9 @@ int ensure_wide(Yue2Model& m) {
   if ((rc = m.alloc(&a, kMaxWideRows * sizeof(DevRow))) || (rc = m.alloc(&b, kMaxWideRows * V * 4)) ||
       (rc = m.alloc(&c, kMaxWideRows * ((V + 7) & ~(size_t)7) * 2)))
     return rc;
-  CK(cudaMemset(a, 0, kMaxWideRows * sizeof(DevRow)));
+  // on the model's stream: on the default one, which that does not wait for, it could clear the
+  // rows of the first pass after their upload
+  CK(cudaMemsetAsync(a, 0, kMaxWideRows * sizeof(DevRow), m.stream));
   m.wide_rows = (DevRow*)a;
   m.wide_logits = (float*)b;
   m.wide_head = (uint16_t*)c;
