@@ -838,3 +838,27 @@ def test_python_refusals(ops):
             f()
             pytest.fail(f"call {i} was taken")
     ops.check_status()
+
+
+def test_rows_that_ask_for_a_gradient_are_refused(ops):
+    q, k = randn((10, 4, 64), torch.bfloat16, 1), randn((10, 2, 64), torch.bfloat16, 2)
+    cu, pos, slots = offsets([10]), ints(range(10)), ints(range(10), torch.int64)
+    pool = ops.KvPool(randn((2, 1, 2, 2, 64, 64), torch.bfloat16, 3))
+    cos = torch.ones(16, 32, device="cuda")
+    gain = torch.ones(64, device="cuda")
+    qkv = torch.cat([q, k, k], 1)
+
+    def ask(t):
+        return t.clone().requires_grad_()
+
+    calls = [lambda: ops.attention_packed(ask(q), k, k, cu), lambda: ops.attention_packed(q, ask(k), k, cu),
+             lambda: ops.attention_packed(q, k, ask(k), cu), lambda: ops.attention_tree(ask(q), pool, 0, ints([[0, 1]]), ints([0]), cu),
+             lambda: ops.qk_rope_append(ask(qkv), None, None, 1e-6, cos, cos, pos, pool, 0, slots),
+             lambda: ops.qk_rope_append(qkv, ask(gain), gain, 1e-6, cos, cos, pos, pool, 0, slots),
+             lambda: ops.qk_rope_append(qkv, gain, ask(gain), 1e-6, cos, cos, pos, pool, 0, slots)]
+    for f in calls:
+        with pytest.raises(Yue2Error, match="gradient"):
+            f()
+        with torch.no_grad():
+            f()
+    ops.check_status()

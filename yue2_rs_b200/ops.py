@@ -6,7 +6,8 @@ Every call runs on the current stream of its tensors' device, allocates through 
 (outputs and workspaces) and can be captured into a CUDA graph: lengths, page tables and
 lists are read on the device. Sizes, types and strides are checked at once (Yue2Error); what
 only the device sees (page indexes, lengths, positions) is checked there, an entry out of
-range is skipped, and `check_status` reports it.
+range is skipped, and `check_status` reports it. The operators serve: they have no backward
+pass, and refuse rows that ask for one.
 
 A step over a batch of requests: `qk_rope_append` writes the new rows' K and V into the pages,
 `attention_packed` attends over whole prompts, `attention_tree` checks drafted tokens against
@@ -117,11 +118,18 @@ def _table(t, dtype, index, what):
     raise _invalid(f"{what} must be a contiguous two-dimensional tensor of {dtype} on cuda:{index}")
 
 
+def _no_gradient(what):
+    if torch.is_grad_enabled():
+        raise _invalid(f"{what} asks for a gradient, which these operators do not have: call them under torch.no_grad()")
+
+
 def _rows(t, index, dtype, what, shape=None):
     """The address, row stride and shape of a [rows, heads, dim] tensor with adjacent heads."""
     if t.dtype is not dtype or t.get_device() != index or t.dim() != 3 or (shape is not None and t.shape != shape):
         raise _invalid(f"{what} must be a [rows, heads, dim] tensor of {dtype} on cuda:{index}"
                        + (f" of shape {tuple(shape)}" if shape is not None else ""))
+    if t.requires_grad:
+        _no_gradient(what)
     rows, heads, dim = t.shape
     step, head, one = t.stride()
     if (one != 1 or (heads > 1 and head != dim)) and rows and heads and dim:
@@ -169,6 +177,8 @@ def qk_rope_append(qkv, q_norm, k_norm, eps, cos, sin, positions, pool, layer, s
         raise _invalid("cos and sin must be [table rows, dim / 2]")
     if (q_norm is None) != (k_norm is None):
         raise _invalid("q_norm and k_norm go together")
+    if q_norm is not None and (q_norm.requires_grad or k_norm.requires_grad):
+        _no_gradient("the norm")
     if q_out is None:
         q_out = qkv.new_empty((rows, heads, dim))
         qp, qs = q_out.data_ptr(), heads * dim
