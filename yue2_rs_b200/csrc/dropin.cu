@@ -175,7 +175,7 @@ uint16_t* weight(DropIn& d, const uint8_t* raw, size_t mapping, size_t rows, siz
   if (!ok_or(cudaMalloc(&dev, n * 2), "weight upload")) return nullptr;
   cudaError_t e;
   if (dtype == YUE2_DTYPE_BF16) {
-    e = cudaMemcpy(dev, raw, n * 2, cudaMemcpyHostToDevice);
+    e = cudaMemcpyAsync(dev, raw, n * 2, cudaMemcpyHostToDevice, d.stream);
   } else {
     std::vector<uint16_t> h(n);
     for (size_t i = 0; i < n; ++i) {
@@ -192,7 +192,7 @@ uint16_t* weight(DropIn& d, const uint8_t* raw, size_t mapping, size_t rows, siz
       }
       h[i] = (uint16_t)(det_f2u(round_bf16(f)) >> 16);
     }
-    e = cudaMemcpy(dev, h.data(), n * 2, cudaMemcpyHostToDevice);
+    e = cudaMemcpyAsync(dev, h.data(), n * 2, cudaMemcpyHostToDevice, d.stream);
   }
   if (!ok_or(e, "weight upload")) {
     cudaFree(dev);
@@ -208,7 +208,7 @@ float* norm(DropIn& d, const float* host, size_t len) {
   if (it != d.norms.end()) return it->second;
   float* dev = nullptr;
   if (!ok_or(cudaMalloc(&dev, len * 4), "norm upload")) return nullptr;
-  if (!ok_or(cudaMemcpy(dev, host, len * 4, cudaMemcpyHostToDevice), "norm upload")) {
+  if (!ok_or(cudaMemcpyAsync(dev, host, len * 4, cudaMemcpyHostToDevice, d.stream), "norm upload")) {
     cudaFree(dev);
     return nullptr;
   }
@@ -244,7 +244,7 @@ Context* context(DropIn& d, const float* k, const float* v, size_t keys, size_t 
       return nullptr;
     }
     if (!ok_or(cudaMalloc(&c.d_pages, npages * 8), "page table") ||
-        !ok_or(cudaMemcpy(c.d_pages, c.pages.data(), npages * 8, cudaMemcpyHostToDevice), "page table")) {
+        !ok_or(cudaMemcpyAsync(c.d_pages, c.pages.data(), npages * 8, cudaMemcpyHostToDevice, d.stream), "page table")) {
       drop_context(d, c);
       return nullptr;
     }

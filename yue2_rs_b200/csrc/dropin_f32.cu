@@ -285,7 +285,7 @@ float* weight_f32(F32Ctx& c, const uint8_t* raw, size_t mapping, size_t rows, si
   }
   float* dev = nullptr;
   if (!f_ok(cudaMalloc(&dev, n * 4), "weight upload")) return nullptr;
-  if (!f_ok(cudaMemcpy(dev, h.data(), n * 4, cudaMemcpyHostToDevice), "weight upload")) {
+  if (!f_ok(cudaMemcpyAsync(dev, h.data(), n * 4, cudaMemcpyHostToDevice, c.stream), "weight upload")) {
     cudaFree(dev);
     return nullptr;
   }
@@ -564,7 +564,7 @@ int yue2_cuda_stack(const float* input, float* out, const Yue2GpuLayer* layers, 
           pre[prefix * kw + i] = (uint16_t)(det_f2u(L.value[i]) >> 16);
         }
         if (!f_ok(cudaMalloc(&pb, pre.size() * 2), "prefix upload") ||
-            !f_ok(cudaMemcpy(pb, pre.data(), pre.size() * 2, cudaMemcpyHostToDevice), "prefix upload"))
+            !f_ok(cudaMemcpyAsync(pb, pre.data(), pre.size() * 2, cudaMemcpyHostToDevice, x.stream), "prefix upload"))
           return 0;
         x.prefixes[key] = pb;
       }

@@ -567,6 +567,7 @@ int yue2_model_finalize(Yue2Model* m) {
     CK(cudaMallocHost(&m->pinned_flags, 4096));
     m->workspace_ready = true;
   }
+  CK(cudaStreamSynchronize(nullptr));  // the weights and tables above, before this model's stream reads them
   m->finalized = true;
   return 0;
 }
@@ -596,7 +597,9 @@ int yue2_cache_create(Yue2Model* m, uint64_t capacity, Yue2Cache** out) {
     return rc;
   }
   c->d_pages = (uint64_t*)pt;
-  cudaError_t e = cudaMemcpy(c->d_pages, c->pages.data(), npages * 8, cudaMemcpyHostToDevice);
+  // On the model's stream, as everything that its passes read: a small copy on the default stream
+  // may still be under way when the call returns, and this stream does not wait for that one.
+  cudaError_t e = cudaMemcpyAsync(c->d_pages, c->pages.data(), npages * 8, cudaMemcpyHostToDevice, m->stream);
   if (e != cudaSuccess) {
     yue2_cache_free(c);
     return cuda_fail(e, "page table upload");
@@ -1127,7 +1130,7 @@ int yue2_prefill(Yue2Model* m, Yue2Cache* c, const int64_t* ids, uint64_t n, int
   void* ids_mem = nullptr;
   if ((rc = m->scratch_take(&ids_mem, n * 4))) return rc;
   int32_t* d_ids = (int32_t*)ids_mem;
-  cudaError_t e = cudaMemcpy(d_ids, h.data(), n * 4, cudaMemcpyHostToDevice);
+  cudaError_t e = cudaMemcpyAsync(d_ids, h.data(), n * 4, cudaMemcpyHostToDevice, m->stream);
   if (e != cudaSuccess) {
     m->scratch_give(d_ids);
     return cuda_fail(e, "prefill ids");

@@ -109,7 +109,7 @@ struct SamplerBufs {
     if (need_words && (rc = get((void**)&words, n * 2 * V * 4))) return rc;
     if ((rc = get((void**)&acc, n * sizeof(SampleAcc)))) return rc;
     std::vector<SampleAcc> zero(n, SampleAcc{0, 0, ~0ull});
-    if (cudaMemcpy(acc, zero.data(), n * sizeof(SampleAcc), cudaMemcpyHostToDevice) != cudaSuccess) {
+    if (cudaMemcpyAsync(acc, zero.data(), n * sizeof(SampleAcc), cudaMemcpyHostToDevice, m->stream) != cudaSuccess) {
       cudaGetLastError();
       return fail(YUE2_ERR_CUDA, "sampler accumulator initialisation failed");
     }
@@ -189,7 +189,8 @@ int yue2_rng_create(Yue2Model* m, uint64_t seed, Yue2Rng** out) {
     delete r;
     return cuda_fail(e, "rng state");
   }
-  if ((e = cudaMemcpy(r->state, &h, sizeof(h), cudaMemcpyHostToDevice)) != cudaSuccess) {
+  if ((e = cudaMemcpyAsync(r->state, &h, sizeof(h), cudaMemcpyHostToDevice, m->stream)) != cudaSuccess ||
+      (e = cudaStreamSynchronize(m->stream)) != cudaSuccess) {
     yue2_rng_free(r);
     return cuda_fail(e, "rng state upload");
   }
@@ -235,8 +236,8 @@ int yue2_choose(Yue2Model* m, const float* logits, uint64_t vocab, const Yue2Sam
   if ((rc = b.alloc(m, 1, vocab, hlen + 1, draw))) return rc;
   float* d_logits = nullptr;
   if ((rc = b.get((void**)&d_logits, vocab * 4))) return rc;
-  CK(cudaMemcpy(d_logits, logits, vocab * 4, cudaMemcpyHostToDevice));
-  CK(cudaMemcpy(b.tokens, hist.data(), hist.size() * 4, cudaMemcpyHostToDevice));
+  CK(cudaMemcpyAsync(d_logits, logits, vocab * 4, cudaMemcpyHostToDevice, m->stream));
+  CK(cudaMemcpyAsync(b.tokens, hist.data(), hist.size() * 4, cudaMemcpyHostToDevice, m->stream));
   SampleReq q = {};
   q.cond_row = 0;
   q.uncond_row = -1;
@@ -248,9 +249,9 @@ int yue2_choose(Yue2Model* m, const float* logits, uint64_t vocab, const Yue2Sam
   q.last = -1;
   q.bookkeeping = 0;
   q.tokens = b.tokens;
-  CK(cudaMemcpy(b.reqs, &q, sizeof(q), cudaMemcpyHostToDevice));
+  CK(cudaMemcpyAsync(b.reqs, &q, sizeof(q), cudaMemcpyHostToDevice, m->stream));
   const int32_t live[2] = {1, 0};
-  CK(cudaMemcpy(b.flags, live, 8, cudaMemcpyHostToDevice));
+  CK(cudaMemcpyAsync(b.flags, live, 8, cudaMemcpyHostToDevice, m->stream));
   if (draw) {
     // the MT kernel advances rng->state by 2*vocab words (sampling.rs:198-213)
     CK(launch_mt_words(m->stream, rng->state, b.words, (int)(2 * vocab), b.reqs, 1));
@@ -344,7 +345,7 @@ int yue2_session_create(Yue2Model* m, const Yue2Sampling* s, int phase, const Yu
       }
       d_prompts.push_back(d);
       cudaError_t e;
-      if ((e = cudaMemcpy(d, h.data(), len * 4, cudaMemcpyHostToDevice)) != cudaSuccess) {
+      if ((e = cudaMemcpyAsync(d, h.data(), len * 4, cudaMemcpyHostToDevice, m->stream)) != cudaSuccess) {
         free_prompts();
         return bail(cuda_fail(e, "prompt upload"));
       }
@@ -392,10 +393,10 @@ int yue2_session_create(Yue2Model* m, const Yue2Sampling* s, int phase, const Yu
     q.tokens = ss->bufs.tokens + i * s->max_tokens;
     mt_seed(hm[i], reqs[i].seed);
   }
-  CK(cudaMemcpy(ss->bufs.reqs, hq.data(), n * sizeof(SampleReq), cudaMemcpyHostToDevice));
-  CK(cudaMemcpy(ss->bufs.mt, hm.data(), n * sizeof(MtState), cudaMemcpyHostToDevice));
+  CK(cudaMemcpyAsync(ss->bufs.reqs, hq.data(), n * sizeof(SampleReq), cudaMemcpyHostToDevice, m->stream));
+  CK(cudaMemcpyAsync(ss->bufs.mt, hm.data(), n * sizeof(MtState), cudaMemcpyHostToDevice, m->stream));
   const int32_t flags[2] = {(int32_t)n, 0};
-  CK(cudaMemcpy(ss->bufs.flags, flags, 8, cudaMemcpyHostToDevice));
+  CK(cudaMemcpyAsync(ss->bufs.flags, flags, 8, cudaMemcpyHostToDevice, m->stream));
   // decode rows: one new token per cache per step
   std::vector<DevRow> rows(R);
   for (int r = 0; r < R; ++r) {

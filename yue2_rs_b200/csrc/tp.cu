@@ -145,7 +145,7 @@ int yue2_tp_connect(Yue2Model* m, const void* handles) {
   }
   void* d = nullptr;
   if ((rc = m->alloc(&d, sizeof(TpPeers)))) return rc;
-  CK(cudaMemcpy(d, &peers, sizeof(TpPeers), cudaMemcpyHostToDevice));
+  CK(cudaMemcpyAsync(d, &peers, sizeof(TpPeers), cudaMemcpyHostToDevice, m->stream));
   m->tp_peers = (TpPeers*)d;
   m->tp_connected = true;
   return 0;
