@@ -397,7 +397,8 @@ int yue2_qk_rope_append(const void* qkv, uint64_t rows, uint64_t heads, uint64_t
 
 /* Attention over whole packed sequences: rows cu[s] .. cu[s+1] - 1 of q [tokens, heads, dim],
  * k and v [tokens, kv, dim] are sequence s (cu: int32 [seqs + 1], nondecreasing, empty
- * sequences allowed; at most 1,024 sequences and 262,144 tokens). A row sees the rows of its
+ * sequences allowed; at most 1,024 sequences and 262,144 tokens; sequences that overlap to more
+ * than `tokens` rows in all: YUE2_STATUS_RANGE and no output). A row sees the rows of its
  * sequence up to itself (causal != 0) or all of them; out = softmax(scale q.k) v in `dtype`.
  * Rows of `out` outside [cu[0], cu[seqs]) are left as they were, and what a masked position or a
  * row outside the sequence holds (infinities and NaN included) reaches no output. `out` may be

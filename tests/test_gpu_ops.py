@@ -276,6 +276,16 @@ def test_packed_bad_offsets_are_reported(ops, cu):
     ops.check_status()
 
 
+def test_packed_offsets_that_go_back_and_forth_do_nothing(ops):
+    # each second sequence is valid by itself, together they are more rows than there are
+    q, k = randn((300, 2, 64), torch.bfloat16, 1), randn((300, 1, 64), torch.bfloat16, 2)
+    out = torch.full_like(q, 7.0)
+    ops.attention_packed(q, k, k, ints([0, 300] * 8), out=out)
+    with pytest.raises(Yue2Error, match="out of range"):
+        ops.check_status()
+    assert bool((out == 7.0).all())
+
+
 # ------------------------------------------------------------------ drafted tokens over pages
 def make_pages(rng, need, extra=3):
     """Shuffled page tables for sequences of need[s] positions; unused entries point far away."""

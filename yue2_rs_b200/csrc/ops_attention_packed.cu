@@ -94,14 +94,17 @@ Y2_DEV int count_above(const PackedArgs& a, int level) {
 }
 Y2_DEV void walk_begin(const PackedArgs& a, Walk& w) {
   const int lane = threadIdx.x & 31;
-  int most = 0;
+  int most = 0, sum = 0;  // at most 2^10 sequences of 2^18 rows
   bool bad = false;
   for (int s = lane; s < a.seqs; s += 32) {
     bad |= seq_of(a, s).n < 0;
+    sum += max(0, seq_of(a, s).n);
     most = max(most, blocks_of(a, s));
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+  most = __reduce_max_sync(0xffffffffu, most);
+  // offsets that go back and forth would give more rows than there are, up to hundreds of times
+  // the work of any valid call: none is done
+  if (__reduce_add_sync(0xffffffffu, sum) > a.tokens) bad = true, most = 0;
   if (bad && blockIdx.x == 0) status_or(a.status, YUE2_STATUS_RANGE);
   w.level = most - 1;
   w.base = 0;
