@@ -1,0 +1,113 @@
+"""Attention scores of -inf and close to the ends of f32, against plain 64-bit forms.
+
+A key whose score is -inf has no weight, and a row without any weight is zero (as a row that sees
+nothing). The tolerances are those of test_gpu_ops.attend over the keys that keep a weight: the
+places that make a score infinite are taken out of the reference's keys before its products."""
+import math
+import random
+
+import numpy as np
+import pytest
+import torch
+
+from test_gpu_ops import DEV, attend, close, ints, make_pages, offsets, ops, randn  # noqa: F401 (ops is a fixture)
+
+pytestmark = pytest.mark.gpu
+
+C = 3  # the component that makes scores infinite; the queries' is positive there
+LOWEST = torch.finfo(torch.bfloat16).min
+
+
+def rows_of(n, heads, dim, dtype, seed):
+    q = randn((n, heads, dim), dtype, seed)
+    q[:, :, C] = q[:, :, C].abs() + 0.5
+    return q
+
+
+def reference(q, k, v, gone, see, scale):
+    """Output and tolerance of rows q [n, heads, dim] over k and v [m, kv, dim]; the keys `gone` [m, kv]
+    have no weight."""
+    heads, kv = q.shape[1], k.shape[1]
+    want = torch.zeros(q.shape, dtype=torch.float64, device=q.device)
+    tol = torch.zeros_like(want)
+    for h in range(heads):
+        g = h // (heads // kv)
+        lives = ~gone[:, g]
+        kk = torch.where(lives[:, None], k[:, g], torch.zeros_like(k[:, g]))
+        vv = torch.where(lives[:, None], v[:, g], torch.zeros_like(v[:, g]))
+        want[:, h], tol[:, h] = attend(q[:, h], kk, vv, see & lives[None], scale)
+    return want, tol
+
+
+def sees(n, causal):
+    i = torch.arange(n, device=DEV)
+    return i[None] <= i[:, None] if causal else torch.ones((n, n), dtype=torch.bool, device=DEV)
+
+
+def check_packed(ops, lens, dropped, causal, dtype, dim, rows=slice(None), heads=4, kv=2, low=0.0, huge=None):
+    """`dropped`: keys of every sequence whose scores are -inf; `low` shifts all other scores."""
+    n = sum(lens)
+    q, k, v = rows_of(n, heads, dim, dtype, 1), randn((n, kv, dim), dtype, 2), randn((n, kv, dim), dtype, 3)
+    if low:
+        q[:, :, 5], k[:, :, 5] = 8, low
+    gone = torch.zeros((n, kv), dtype=torch.bool, device=DEV)
+    at = 0
+    for m in lens:
+        keys = [at + j for j in dropped if j < m]
+        gone[keys] = True
+        at += m
+    k[..., C] = torch.where(gone, -math.inf, k[..., C])
+    if huge is not None:
+        v[gone] = huge
+    got = ops.attention_packed(q, k, v, offsets(lens), causal=causal)
+    ops.check_status()
+    at = 0
+    for m in lens:
+        part = slice(at, at + m)
+        want, tol = reference(q[part], k[part], v[part], gone[part], sees(m, causal), 1 / math.sqrt(dim))
+        close(got[part][rows], want[rows], tol[rows], (m, causal))
+        at += m
+
+
+@pytest.mark.parametrize("low", [0.0, -200.0])  # -200: scores far below what 2^x holds relative to zero
+@pytest.mark.parametrize("dim,dtype", [(64, torch.float16), (128, torch.bfloat16)])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("tiles", [1, 2])
+def test_packed_first_tiles_without_a_weight(ops, tiles, causal, dim, dtype, low):
+    # the rows behind them see ordinary scores in several tiles, first below and then above any
+    # score so far
+    check_packed(ops, [317 + 128 * tiles, 900, 640], range(128 * tiles), causal, dtype, dim, slice(128 * tiles, None), low=low)
+
+
+def check_tree(ops, ctx, nodes, dropped, dtype, dim, heads=6, kv=2, mask=None, huge=None, scale=None, value=-math.inf):
+    """One call over sequences of ctx[s] positions and nodes[s] drafted ones; dropped(s, n): its keys
+    whose scores are -inf."""
+    rng = random.Random(7)
+    held = [c + t for c, t in zip(ctx, nodes)]
+    pages, table = make_pages(rng, held)
+    data = randn((pages, 1, 2, kv, 64, dim), dtype, 4)
+    q = rows_of(sum(nodes), heads, dim, dtype, 5)
+    expect, at = [], 0
+    for s, (c, t) in enumerate(zip(ctx, nodes)):
+        pos = torch.arange(c + t, device=DEV)
+        page = ints(table[s]).long()[pos // 64]
+        gone = torch.zeros(c + t, dtype=torch.bool, device=DEV)
+        gone[list(dropped(s, c + t))] = True
+        data[page[gone], 0, 0, :, pos[gone] % 64, C] = value
+        if huge is not None:
+            data[page[gone], 0, 1, :, pos[gone] % 64] = huge
+        k, v = data[page, 0, 0, :, pos % 64], data[page, 0, 1, :, pos % 64]
+        see = pos[None] <= c + torch.arange(t, device=DEV)[:, None]
+        expect.append((slice(at, at + t), q[at:at + t], k, v, gone[:, None].expand(-1, kv), see))
+        at += t
+    got = ops.attention_tree(q, ops.KvPool(data), 0, ints(table), ints(ctx), offsets(nodes), scale=scale)
+    ops.check_status()
+    for rows, qq, k, v, gone, see in expect:
+        want, tol = reference(qq, k, v, gone, see, 1 / math.sqrt(dim) if scale is None else scale)
+        close(got[rows], want, tol, rows)
+
+
+@pytest.mark.parametrize("dim,dtype", [(64, torch.float16), (128, torch.bfloat16)])
+@pytest.mark.parametrize("ctx,nodes", [([700], [3]), ([5000, 300], [1, 9]), ([700], [64])])
+def test_tree_first_tiles_without_a_weight(ops, ctx, nodes, dim, dtype):
+    check_tree(ops, ctx, nodes, lambda s, n: range(256), dtype, dim)

@@ -361,12 +361,14 @@ Y2_DEV void softmax_masked(uint32_t s_addr, uint32_t o_addr, float c, bool negat
 // The same for a tile that every row sees whole, with a positive scale, after the first one: the
 // weights are formed relative to the m there is, the maximum is found on the way, and only
 // when it asks for another m (false: nothing has been written) softmax_masked does the tile.
+// The vote also turns down an m without a finite c m: after tiles without any weight (scores of
+// -inf) m is -inf, which no weight can be taken relative to.
 // Without the first pass the exponentials start as soon as the scores are there (8,192 rows of
 // 24 heads, all seen: 756 -> 716 us). Only long packed sequences gain: in tree attention
 // the larger code costs more than the pass (full trees 65.2 -> 67.8 us).
 template <int D, bool F16, class Part>
 Y2_DEV bool softmax_settled(uint32_t s_addr, float c, RowStats& st, Part part) {
-  const float mc = exponent_base(c, st);
+  const float cm = -st.m * c, mc = fabsf(cm) < INFINITY ? cm : NAN;
   uint32_t v[2][32], p[3][16];
   float l[4] = {0.f, 0.f, 0.f, 0.f}, mx = -INFINITY, my = -INFINITY;
   auto weights = [&](float a, float b, int i, float (&sum)[4]) {
