@@ -400,10 +400,10 @@ int yue2_qk_rope_append(const void* qkv, uint64_t rows, uint64_t heads, uint64_t
  * sequences allowed; at most 1,024 sequences and 262,144 tokens; sequences that overlap to more
  * than `tokens` rows in all: YUE2_STATUS_RANGE and no output). A row sees the rows of its
  * sequence up to itself (causal != 0) or all of them; out = softmax(scale q.k) v in `dtype`.
- * Rows of `out` outside [cu[0], cu[seqs]) are left as they were, and what a masked position or a
- * row outside the sequence holds (infinities and NaN included) reaches no output. `out` may be
- * q itself (same base and stride) and overlaps neither k nor v. dim 64 or 128, heads a
- * multiple of kv. */
+ * A key whose score is -inf has no weight, and a row of such keys alone is zero. Rows of `out`
+ * outside [cu[0], cu[seqs]) are left as they were, and what a masked position or a row outside
+ * the sequence holds (infinities and NaN included) reaches no output. `out` may be q itself
+ * (same base and stride) and overlaps neither k nor v. dim 64 or 128, heads a multiple of kv. */
 int yue2_attention_packed(const void* q, const void* k, const void* v, void* out, const int32_t* cu, uint64_t seqs,
                           uint64_t tokens, uint64_t heads, uint64_t kv, uint64_t dim, uint64_t q_stride,
                           uint64_t k_stride, uint64_t v_stride, uint64_t out_stride, int32_t dtype, int32_t causal,
@@ -414,10 +414,10 @@ int yue2_attention_packed(const void* q, const void* k, const void* v, void* out
  * whose K/V are already in the pages (yue2_qk_rope_append). Row cu[s] + i of q [rows, heads,
  * dim] sees the whole context and the drafted positions context[s] + j whose bit j is set in
  * mask[cu[s] + i] (a node's ancestors and itself; bits >= T are ignored); mask NULL: j <= i,
- * so T = 1 is an ordinary decode step. A row that sees nothing gets zeros; rows of `out`
- * outside [cu[0], cu[seqs]) are left as they were; what a masked or unused place of a page holds
- * reaches no output; a sequence with a bad page index has undefined outputs. `out` does not
- * overlap q. At most 1,024 sequences and 128 query heads per kv head, and a pool of fewer
+ * so T = 1 is an ordinary decode step. A row that sees nothing, or scores of -inf alone, gets
+ * zeros; rows of `out` outside [cu[0], cu[seqs]) are left as they were; what a masked or unused
+ * place of a page holds reaches no output; a sequence with a bad page index has undefined
+ * outputs. `out` does not overlap q. At most 1,024 sequences and 128 query heads per kv head, and a pool of fewer
  * than 2^31 [dim] rows. `workspace`:
  * yue2_attention_tree_workspace bytes (0: may be NULL), 16-byte aligned, contents free before
  * and after; calls that may overlap need their own. */

@@ -111,3 +111,36 @@ def check_tree(ops, ctx, nodes, dropped, dtype, dim, heads=6, kv=2, mask=None, h
 @pytest.mark.parametrize("ctx,nodes", [([700], [3]), ([5000, 300], [1, 9]), ([700], [64])])
 def test_tree_first_tiles_without_a_weight(ops, ctx, nodes, dim, dtype):
     check_tree(ops, ctx, nodes, lambda s, n: range(256), dtype, dim)
+
+
+@pytest.mark.parametrize("dtype,huge,dim", [(torch.bfloat16, 3.0e38, 128), (torch.float16, 65504.0, 64)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_packed_single_keys_without_a_weight_add_nothing(ops, causal, dtype, huge, dim):
+    # at places of either way of exponentials, their values as large as the type holds them
+    check_packed(ops, [600, 1, 512], [0, 14, 15, 31, 62, 130, 142, 143, 158, 159, 254, 300, 399, 511], causal, dtype, dim, huge=huge)
+
+
+@pytest.mark.parametrize("dtype,huge,dim", [(torch.bfloat16, 3.0e38, 128), (torch.float16, 65504.0, 64)])
+@pytest.mark.parametrize("nodes", [1, 20, 64])
+def test_tree_single_keys_without_a_weight_add_nothing(ops, nodes, dtype, huge, dim):
+    places = [0, 14, 15, 31, 62, 130, 142, 143, 158, 159, 254, 300, 399, 511]
+    check_tree(ops, [600, 2000], [nodes, 3], lambda s, n: places, dtype, dim, huge=huge)
+
+
+@pytest.mark.parametrize("dtype,dim", [(torch.bfloat16, 128), (torch.float16, 64)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_packed_rows_without_any_weight_are_zero(ops, causal, dtype, dim):
+    check_packed(ops, [1, 100, 128, 300, 512], range(512), causal, dtype, dim)
+    if causal:  # and rows with a weight in the same tiles
+        check_packed(ops, [200, 517], range(150), causal, dtype, dim)
+
+
+@pytest.mark.parametrize("dtype,dim", [(torch.bfloat16, 128), (torch.float16, 64)])
+def test_tree_rows_without_any_weight_are_zero(ops, dtype, dim):
+    # items of one share and items that are cut, rows of one side and of two; then other sequences
+    # of the same call with ordinary scores
+    check_tree(ops, [0, 5, 128, 700], [1, 64, 9, 64], lambda s, n: range(n), dtype, dim)
+    check_tree(ops, [9000], [2], lambda s, n: range(n), dtype, dim)
+    check_tree(ops, [9000, 3000, 40], [40, 2, 1], lambda s, n: range(n) if s < 2 else [], dtype, dim)
+    # cut items whose first shares have no weight
+    check_tree(ops, [9000], [2], lambda s, n: range(4000), dtype, dim)

@@ -250,8 +250,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!__all_sync(0xffffffffu, wait(o_full + side, o_phase, ending, a.status))) break;
         o_phase ^= 1;
         tc::fence_after();
-        const float inv = 1.0f / st.total();
-        const bool found = *(volatile int*)&units[us].found;
+        const float l = st.total(), inv = 1.0f / l;
+        const bool some = l != 0.f;  // else every score is -inf: zeros
+        const bool found = some && *(volatile int*)&units[us].found;
         char* to[4];
         quad_rows(t < rows ? a.out + (long long)(u.first + row) * a.out_stride + u.head * D : nullptr, to);
 #pragma unroll 1
@@ -262,7 +263,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           arrived(o);
           float f[32];
 #pragma unroll
-          for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(o[i]) * inv;
+          for (int i = 0; i < 32; ++i) f[i] = some ? __uint_as_float(o[i]) * inv : 0.f;
           if (found && t < rows)  // keys of the unit's masked tiles that this row sees
             for (int key = u.block * kBlock; key <= last; ++key)
               add_nonfinite<F16>(a.v + (long long)(u.first + key) * a.v_stride + (u.head / a.group) * D + 32 * q, f);

@@ -281,7 +281,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (warp_live && (side == 0 || !turns)) {
         const bool found = *(volatile int*)&units[us].found;
-        const float inv = l > 0.f ? 1.0f / l : l == 0.f ? 0.f : l;  // nothing seen: zeros
+        const float inv = 1.0f / l;
+        const bool some = l != 0.f;  // else nothing seen, or scores of -inf alone: zeros
         const int row = u.first + node, head = u.head * a.group + t % a.group;
         const long long prow = (long long)u.slot * a.slot_rows + (node - u.node) * a.group + t % a.group;
         void* mine = u.slot >= 0 ? (void*)(a.part + prow * D) : (void*)(a.out + (long long)row * a.out_stride + (long long)head * D);
@@ -330,7 +331,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           } else {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) f[i] *= inv;
+            for (int i = 0; i < 32; ++i) f[i] = some ? f[i] * inv : 0.f;
             pack32<F16>(f, v);
             quad_store(to, 64 * q, v);
           }
@@ -635,10 +636,12 @@ __global__ void __launch_bounds__(kMergeThreads, 6) tree_merge_kernel(const Tree
     }
   }
   l = warp_sum(l);
-  const float inv = l > 0.f ? 1.0f / l : l == 0.f ? 0.f : l;
+  const float inv = 1.0f / l;
   uint16_t* dst = a.out + (long long)row * a.out_stride + (long long)h * D + lane * E;
 #pragma unroll
-  for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = pack16<F16>(o[e] * inv, o[e + 1] * inv);
+  for (int e = 0; e < E; ++e) o[e] = l != 0.f ? o[e] * inv : 0.f;
+#pragma unroll
+  for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = pack16<F16>(o[e], o[e + 1]);
 }
 
 int sm_count(int& sms) {

@@ -197,9 +197,10 @@ def attention_packed(q, k, v, cu, causal=True, scale=None, out=None):
     """Attention over whole packed sequences: rows cu[s] .. cu[s + 1] - 1 of q [tokens, heads,
     dim], k and v [tokens, kv, dim] are sequence s (cu int32 [seqs + 1]; at most 1,024
     sequences, empty ones allowed, and 262,144 tokens). A row sees its sequence up to itself,
-    or all of it with causal=False. scale: 1 / sqrt(dim) by default. Rows outside
-    [cu[0], cu[-1]) of `out` are left as they were (undefined when `out` is None). bf16 or
-    f16, dim 64 or 128; strided rows are fine."""
+    or all of it with causal=False. scale: 1 / sqrt(dim) by default. A key whose score is -inf
+    has no weight, and a row of such keys alone is zero. Rows outside [cu[0], cu[-1]) of `out`
+    are left as they were (undefined when `out` is None). bf16 or f16, dim 64 or 128; strided
+    rows are fine."""
     dev, dtype = q.get_device(), q.dtype
     code = _DTYPES.get(dtype)
     if code is None or dev < 0:
@@ -228,8 +229,9 @@ def attention_tree(q, pool, layer, table, context, cu, mask=None, scale=None, ou
     whose K/V are in the pages too; rows cu[s] .. cu[s + 1] - 1 of q [rows, heads, dim] are
     theirs. Row i sees the context and the drafted positions whose bit is set in mask[row]
     (int64: a node's ancestors and itself); mask None: all up to itself, so that one row per
-    sequence is an ordinary decode step. A row that sees nothing gets zeros; rows outside
-    [cu[0], cu[-1]) of `out` are left as they were (undefined when `out` is None)."""
+    sequence is an ordinary decode step. A row that sees nothing, or scores of -inf alone, gets
+    zeros; rows outside [cu[0], cu[-1]) of `out` are left as they were (undefined when `out` is
+    None)."""
     dev, dtype, i32 = pool.index, pool.dtype, torch.int32
     qp, qs, rows, heads, dim = _rows(q, dev, dtype, "q")
     if dim != pool.dim:
