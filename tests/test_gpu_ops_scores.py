@@ -144,3 +144,41 @@ def test_tree_rows_without_any_weight_are_zero(ops, dtype, dim):
     check_tree(ops, [9000, 3000, 40], [40, 2, 1], lambda s, n: range(n) if s < 2 else [], dtype, dim)
     # cut items whose first shares have no weight
     check_tree(ops, [9000], [2], lambda s, n: range(4000), dtype, dim)
+
+
+def test_packed_unmasked_values_that_are_not_finite(ops):
+    # every row sees every value of its sequence, whole tiles and the ragged last one alike
+    for n, at in ((400, 399), (513, 512), (700, 645), (700, 40), (1100, 1030)):
+        q, k, v = randn((n + 90, 4, 128), torch.bfloat16, 1), randn((n + 90, 2, 128), torch.bfloat16, 2), randn((n + 90, 2, 128), torch.bfloat16, 3)
+        clean = ops.attention_packed(q, k, v, offsets([n, 90]), causal=False)
+        v[at, 1, 5] = math.inf
+        v[n:, :, 7] = math.nan  # the sequence behind
+        got = ops.attention_packed(q, k, v, offsets([n, 90]), causal=False)
+        ops.check_status()
+        hit = torch.zeros_like(got, dtype=torch.bool)
+        hit[:n, 2:, 5] = True
+        hit[n:, :, 7] = True
+        assert torch.equal(got[~hit], clean[~hit])
+        assert (got[:n, 2:, 5] == math.inf).all() and torch.isnan(got[n:, :, 7]).all()
+
+
+def test_packed_one_value_that_is_not_finite_costs_little(ops):
+    # a pass over the whole sequence for every row would make the call tens of times as long
+    n = 4001
+    q, k, v = randn((n, 8, 128), torch.bfloat16, 1), randn((n, 8, 128), torch.bfloat16, 2), randn((n, 8, 128), torch.bfloat16, 3)
+    cu, out = offsets([n]), torch.empty_like(q)
+
+    def best():
+        times = []
+        for _ in range(6):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            ops.attention_packed(q, k, v, cu, causal=False, out=out)
+            b.record()
+            torch.cuda.synchronize()
+            times.append(a.elapsed_time(b))
+        return min(times)
+
+    ordinary = best()
+    v[n - 1] = math.nan
+    assert best() < 3 * ordinary

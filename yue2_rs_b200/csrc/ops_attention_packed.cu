@@ -220,7 +220,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (lane == 0) tc::mbar_arrive(b + side);
         };
         // only the last tile of a side has keys that some row does not see; the values of the
-        // last tile of either side are cleaned by both, whichever comes first
+        // last tile of either side are cleaned by both, whichever comes first. Without the causal
+        // mask those are the keys past the end alone, and no row has a value to add later.
         const bool masked = j == tiles - 1 && (a.causal || u.n % kKeys);
         const bool clean = masked || (a.causal && j == tiles - 1 - side);
         const int seen = masked ? last - j * kKeys + 1 : kKeys;  // keys [0, seen) of the tile
@@ -234,9 +235,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           const uint32_t at = kv_count + 2 * j + 1;
           ok = __all_sync(0xffffffffu, wait(kv_full + at % SLOTS, (at / SLOTS) & 1, ending, a.status));
           if (!ok) break;
-          for (int slab = 0; slab < D / 64; ++slab)
-            clean_values<F16>(smem + L::OFF_KV + (at % SLOTS) * TILE + slab * (kKeys * 128), t, j * kKeys + t >= u.n,
-                              &units[us].found);
+          const bool dead = j * kKeys + t >= u.n;
+          for (int slab = 0; (a.causal || dead) && slab < D / 64; ++slab)
+            clean_values<F16>(smem + L::OFF_KV + (at % SLOTS) * TILE + slab * (kKeys * 128), t, dead, &units[us].found);
           tc::fence_proxy_async();
         }
         auto part = [&] { announce(p_part); };
