@@ -194,12 +194,15 @@ Y2_DEV float max3(float a, float b, float c) {
 // 2^x of two values on the FMA units: x = n + f with n the nearest integer and |f| <= 1/2, 2^f by
 // a polynomial fitted for the least relative error (degree 3 for bf16 weights: 7.5e-5, degree
 // 4 for f16: 2.6e-6; the rounding that follows is off by up to 3.9e-3 and 4.9e-4), and n added to its
-// exponent. x is below about 100 and not NaN; below -126 the result is 0, as ex2's, so that a key
-// whose score is -inf adds nothing however large its value is.
+// exponent. x is below about 100 and not NaN. From -127 down the result is 0, so that a key whose
+// score is -inf adds nothing however large its value is: there n = -127 and f = 0, and since both
+// constant terms are below 1 the sum of the exponents is negative, which max() turns into 0. (A
+// select on x instead keeps x alive and spilled 40 to 70 bytes a thread.)
 template <bool F16>
 Y2_DEV void poly_ex2(float& x, float& y) {
   constexpr float kRound = 12582912.f;  // 1.5 * 2^23: adding it leaves n in the low bits
-  const bool no_x = x < -126.f, no_y = y < -126.f;
+  x = fmaxf(x, -127.f);
+  y = fmaxf(y, -127.f);
   float nx = x, ny = y;
   add2(nx, ny, kRound, kRound);
   float rx = nx, ry = ny;
@@ -216,8 +219,8 @@ Y2_DEV void poly_ex2(float& x, float& y) {
     fma2(px, py, px, py, fx, fy, 0x1.62f31cp-1f, 0x1.62f31cp-1f);
     fma2(px, py, px, py, fx, fy, 0x1.fff692p-1f, 0x1.fff692p-1f);
   }
-  x = no_x ? 0.f : __uint_as_float(__float_as_uint(px) + (__float_as_uint(nx) << 23));
-  y = no_y ? 0.f : __uint_as_float(__float_as_uint(py) + (__float_as_uint(ny) << 23));
+  x = __int_as_float(max((int)(__float_as_uint(px) + (__float_as_uint(nx) << 23)), 0));
+  y = __int_as_float(max((int)(__float_as_uint(py) + (__float_as_uint(ny) << 23)), 0));
 }
 
 // A new maximum mn of a row (NaN moves m too; a row that has seen nothing yet stays): m moves, and O
