@@ -10,6 +10,7 @@ import numpy as np
 import pytest
 import torch
 
+from test_gpu_ops import check_packed as packed_as_before
 from test_gpu_ops import DEV, attend, close, ints, make_pages, offsets, ops, randn  # noqa: F401 (ops is a fixture)
 
 pytestmark = pytest.mark.gpu
@@ -182,3 +183,55 @@ def test_packed_one_value_that_is_not_finite_costs_little(ops):
     ordinary = best()
     v[n - 1] = math.nan
     assert best() < 3 * ordinary
+
+
+@pytest.mark.parametrize("scale", [None, 1.0, 5.0, -1.0])
+@pytest.mark.parametrize("causal", [True, False])
+def test_packed_keys_at_the_lowest_value(ops, causal, scale):
+    # scores near the end of f32, whose product with the scale passes it; rows that see nothing
+    # else weigh those keys alike (their scores are one and the same number in 64 bits too)
+    lens, dim, sign = [150, 700], 128, -1.0 if scale is not None and scale < 0 else 1.0
+    n = sum(lens)
+    q, k, v = randn((n, 4, dim), torch.bfloat16, 1), randn((n, 2, dim), torch.bfloat16, 2), randn((n, 2, dim), torch.bfloat16, 3)
+    q[:, :, C] = 1
+    gone = torch.zeros((n, 2), dtype=torch.bool, device=DEV)
+    gone[:140] = True
+    gone[150:150 + 300] = True
+    k[..., C] = torch.where(gone, sign * LOWEST, k[..., C])
+    got = ops.attention_packed(q, k, v, offsets(lens), causal=causal, scale=scale)
+    ops.check_status()
+    at = 0
+    for m in lens:
+        part, see = slice(at, at + m), sees(m, causal)
+        want, tol = reference(q[part], k[part], v[part], gone[part], see, 1 / math.sqrt(dim) if scale is None else scale)
+        alike, alike_tol = reference(torch.zeros_like(q[part]), torch.zeros_like(k[part]), v[part], torch.zeros_like(gone[part]), see, 1.0)
+        only = ~(see & ~gone[part, 0][None]).any(1)
+        want[only], tol[only] = alike[only], alike_tol[only]
+        close(got[part], want, tol, m)
+        at += m
+
+
+@pytest.mark.parametrize("value", [2 * LOWEST / 3, -1.0e12])
+@pytest.mark.parametrize("scale", [None, 1.0, 4.0])
+@pytest.mark.parametrize("nodes", [1, 30, 64])
+def test_tree_keys_at_the_lowest_value(ops, nodes, scale, value):
+    check_tree(ops, [700, 6000], [nodes, 2], lambda s, n: range(300), torch.bfloat16, 128, scale=scale, value=value)
+
+
+@pytest.mark.parametrize("dtype,mag", [(torch.bfloat16, 1.0e3), (torch.bfloat16, 1.0e5), (torch.bfloat16, 1.0e9), (torch.float16, 2.0e3)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_packed_large_scores(ops, causal, dtype, mag):
+    # scores of 10^6 to 10^18, whose product with the scale is rounded by more than the weights' range
+    packed_as_before(ops, [300, 520], 4, 2, 128, dtype, causal, mag=mag)
+
+
+@pytest.mark.parametrize("scale", [1.0, 3.0e38])
+def test_packed_one_score_far_above_all_others(ops, scale):
+    # a score times scale beyond f32: its key has all the weight
+    n, at = 500, 201
+    q, k, v = randn((n, 2, 128), torch.bfloat16, 1), randn((n, 1, 128), torch.bfloat16, 2), randn((n, 1, 128), torch.bfloat16, 3)
+    q[:, :, C], k[at, :, C] = 1, -LOWEST
+    got = ops.attention_packed(q, k, v, offsets([n]), scale=scale)
+    ops.check_status()
+    assert torch.equal(got[at:], v[at].expand(n - at, 2, 128))
+    assert torch.isfinite(got[:at]).all()

@@ -205,7 +205,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int row = u.block * kBlock + side * kRows + t;  // within the sequence
       const int last = a.causal ? min(row, u.n - 1) : u.n - 1;
       RowStats st;
-      st.begin();
+      st.begin(t < rows);
       bool ok = true;
       for (int j = 0; j < tiles; ++j) {
         ok = __all_sync(0xffffffffu, wait(s_full + side, s_phase, ending, a.status));
@@ -464,8 +464,7 @@ extern "C" int yue2_attention_packed(const void* q, const void* k, const void* v
   a.group = (int)(heads / kv);
   a.causal = causal != 0;
   a.negate = scale < 0.f;
-  // not below the smallest normal number: a masked score is -inf, and 0 * -inf is not 0
-  a.c = std::max(std::fabs(scale) * 1.4426950408889634f, 1.17549435e-38f);
+  a.c = opt::weight_scale(scale);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (dim == 64) return f16 ? launch<64, true>(mq, mk, mv, a, st) : launch<64, false>(mq, mk, mv, a, st);
   return f16 ? launch<128, true>(mq, mk, mv, a, st) : launch<128, false>(mq, mk, mv, a, st);

@@ -207,7 +207,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint64_t mask = 0;
       if (live) mask = a.mask ? a.mask[u.first + node] & drafted : (node < 63 ? (2ull << node) - 1 : ~0ull);
       RowStats st;
-      st.begin();
+      st.begin(live);
       bool ok = true;
       for (int i = 0; i < tiles; ++i) {
         const int j = u.t0 + (turns ? side : 0) + i * stride;  // tile of the sequence
@@ -236,13 +236,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (!warp_live) {
           part();
-        } else if (masked || a.negate) {
+        } else if (masked || a.negate || !softmax_tile<D, F16>(s_addr, o_addr, a.c, i == 0, st, part)) {
           uint32_t vis[4];
 #pragma unroll
           for (int q = 0; q < 4; ++q) vis[q] = seen_bits(key0 + 32 * q, u.ctx, mask);
           softmax_masked<D, F16, 1>(s_addr, o_addr, a.c, a.negate, i == 0, vis, st, part);
-        } else {
-          softmax_tile<D, F16>(s_addr, o_addr, a.c, i == 0, st, part);
         }
         announce(p_full);
       }
@@ -274,8 +272,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float2 o = ml[t];
         m = max3(m, o.x, o.x);
         if (m != -INFINITY) {
-          w0 = st.m == -INFINITY ? 0.f : ex2((st.m - m) * a.c);
-          w1 = o.x == -INFINITY ? 0.f : ex2((o.x - m) * a.c);
+          w0 = st.m == -INFINITY ? 0.f : ex2(apart(a.c, st.m, m));
+          w1 = o.x == -INFINITY ? 0.f : ex2(apart(a.c, o.x, m));
         }
         l = l * w0 + o.y * w1;
       }
@@ -618,7 +616,7 @@ __global__ void __launch_bounds__(kMergeThreads, 6) tree_merge_kernel(const Tree
       const float2 s = stats[slot(base + lane)];
       // not below the smallest normal number, so that infinities stay what they are; a share in
       // which the row saw nothing has none
-      f = s.x == -INFINITY ? 0.f : max3(ex2((s.x - m) * a.c), 1.17549435e-38f, 0.f);
+      f = s.x == -INFINITY ? 0.f : max3(ex2(apart(a.c, s.x, m)), 1.17549435e-38f, 0.f);
       l = fmaf(s.y, f, l);
     }
     const int n = min(32, c1 - base + 1);
@@ -760,8 +758,7 @@ int yue2_attention_tree(const void* q, uint64_t rows, uint64_t heads, uint64_t q
   a.negate = scale < 0.f;
   a.ctas = plan.ctas;
   a.slot_rows = plan.slot_rows;
-  // not below the smallest normal number: a masked score is -inf, and 0 * -inf is not 0
-  a.c = std::max(std::fabs(scale) * 1.4426950408889634f, 1.17549435e-38f);
+  a.c = opt::weight_scale(scale);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool merge = plan.bytes > 0;
   if (dim == 64) return f16 ? launch<64, true>(mq, mkv, a, merge, st) : launch<64, false>(mq, mkv, a, merge, st);

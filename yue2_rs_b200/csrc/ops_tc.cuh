@@ -8,7 +8,9 @@
 #pragma once
 #include <cudaTypedefs.h>
 
+#include <algorithm>
 #include <atomic>
+#include <cmath>
 
 #include "ops.cuh"
 #include "tcgen05.cuh"
@@ -161,10 +163,12 @@ Y2_DEV float ex2(float x) {
 }
 
 // The running statistics of a thread's row: m is the score that the exponent is taken
-// relative to (not always the maximum so far, see softmax_tile), l the sum of the weights in parts.
+// relative to (not always the maximum so far, see move_max), l the sum of the weights in parts.
+// live: the lane's row is one of the call's (the others hold anything and decide nothing).
 struct RowStats {
   float m, l[4];
-  Y2_DEV void begin() { m = -INFINITY, l[0] = l[1] = l[2] = l[3] = 0.f; }
+  bool live;
+  Y2_DEV void begin(bool is_live) { m = -INFINITY, l[0] = l[1] = l[2] = l[3] = 0.f, live = is_live; }
   Y2_DEV float total() const { return (l[0] + l[1]) + (l[2] + l[3]); }
 };
 
@@ -182,6 +186,14 @@ Y2_DEV void add2(float& x, float& y, float a, float b) {
       "add.rn.f32x2 s, s, t;\n\tmov.b64 {%0, %1}, s;\n\t}"
       : "+f"(x), "+f"(y)
       : "f"(a), "f"(b));
+}
+
+Y2_DEV void mul2(float& x, float& y, float a) {
+  asm("{\n\t.reg .b64 s, t;\n\t"
+      "mov.b64 s, {%0, %1};\n\tmov.b64 t, {%2, %2};\n\t"
+      "mul.rn.f32x2 s, s, t;\n\tmov.b64 {%0, %1}, s;\n\t}"
+      : "+f"(x), "+f"(y)
+      : "f"(a));
 }
 
 // The largest of three, NaN if one of them is.
@@ -223,6 +235,10 @@ Y2_DEV void poly_ex2(float& x, float& y) {
   y = __int_as_float(max((int)(__float_as_uint(py) + (__float_as_uint(ny) << 23)), 0));
 }
 
+// c (a - b), whose difference may pass the end of f32 where the product does not (scores near it, a
+// scale near 0). c is at most a quarter of the largest number.
+Y2_DEV float apart(float c, float a, float b) { return fmaf(a, 0.25f, -0.25f * b) * (4.0f * c); }
+
 // A new maximum mn of a row (NaN moves m too; a row that has seen nothing yet stays): m moves, and O
 // and l are scaled by 2^(c (m_old - m_new)), only when a score exceeds m by more than a factor
 // 2^8 of weight: until then the weights are at most 2^8, exact in the f32 sums, and the final
@@ -230,9 +246,9 @@ Y2_DEV void poly_ex2(float& x, float& y) {
 // previous tile was issued before the scores of this one.
 template <int D>
 Y2_DEV void move_max(uint32_t o_addr, float c, bool first, float mn, RowStats& st) {
-  const bool move = first || (mn != -INFINITY && !((mn - st.m) * c <= 8.0f));
+  const bool move = first || (st.live && mn != -INFINITY && !(apart(c, mn, st.m) <= 8.0f));
   if (!first && __any_sync(0xffffffffu, move)) {
-    const float alpha = move ? ex2((st.m - mn) * c) : 1.0f;
+    const float alpha = move ? ex2(apart(c, st.m, mn)) : 1.0f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) st.l[i] *= alpha;
 #pragma unroll 1
@@ -246,15 +262,27 @@ Y2_DEV void move_max(uint32_t o_addr, float c, bool first, float mn, RowStats& s
   }
   if (move) st.m = mn;
 }
-// -c m, the constant of the exponent. A score of +inf or NaN makes m so and the row NaN.
-Y2_DEV float exponent_base(float c, const RowStats& st) {
-  return st.m == -INFINITY ? 0.f : st.m == INFINITY ? NAN : -st.m * c;
-}
+// Whether c s - c m, one FMA, is the exponent of a score s. c m is rounded, so that all weights of the
+// row share a factor of up to 2^(c m 2^-24), which the division by l removes as long as it fits the
+// weights' type: below 2^20 it is at most 2^(1/16). An infinite or NaN m is out of range, too.
+Y2_DEV bool in_range(float c, float m) { return fabsf(c * m) < 0x1p20f; }
+// The exponent of any row: (a s + b) k. An m of +inf or NaN makes the row NaN; an m of -inf (no score
+// above it yet) gives every weight 0.
+struct Exponent {
+  float a, b, k;
+  Y2_DEV Exponent(float c, float m) {
+    const bool plain = in_range(c, m) || m == -INFINITY;
+    a = plain ? c : 0.25f;
+    b = m == -INFINITY ? 0.f : plain ? -c * m : -0.25f * m;
+    k = plain ? 1.f : 4.f * c;
+  }
+};
 
 // A side's softmax over one tile of 128 keys: the scores in TMEM become weights
-// p = 2^(c (s - m)), packed over them. c = |scale| log2(e). Every lane of the warp takes part.
+// p = 2^(c (s - m)), packed over them. c = |scale| log2(e), weight_scale. Every lane of the warp takes part.
 // The maximum first (m starts as the first tile's), then the weights in a second pass over the
-// scores in TMEM (reading them again costs less than holding 128 registers). p is rounded
+// scores in TMEM (reading them again costs less than holding 128 registers). False, and nothing
+// done, when a row's maximum is out of range: softmax_masked does the tile. p is rounded
 // to 16 bits (relative error of half a step, as the output's own rounding; l sums the
 // unrounded weights). kPoly of 16 pairs take the FMA units, the others the special-function
 // unit, which alone would need as long as the tensor cores (8,192 rows of 24 heads: 719 us
@@ -262,7 +290,7 @@ Y2_DEV float exponent_base(float c, const RowStats& st) {
 // more). part() runs when 96 weights are stored; the caller announces the last 32.
 constexpr int kPoly = 2;
 template <int D, bool F16, class Part>
-Y2_DEV void softmax_tile(uint32_t s_addr, uint32_t o_addr, float c, bool first, RowStats& st, Part part) {
+Y2_DEV bool softmax_tile(uint32_t s_addr, uint32_t o_addr, float c, bool first, RowStats& st, Part part) {
   uint32_t v[2][32];
   float mx[4] = {st.m, st.m, st.m, st.m};
 #pragma unroll
@@ -280,9 +308,11 @@ Y2_DEV void softmax_tile(uint32_t s_addr, uint32_t o_addr, float c, bool first, 
       mx[3] = max3(mx[3], __uint_as_float(v[1][i + 2]), __uint_as_float(v[1][i + 3]));
     }
   }
+  const float mn = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]);
+  if (__any_sync(0xffffffffu, st.live && !in_range(c, mn))) return false;
   load32(s_addr, v[0]);
-  move_max<D>(o_addr, c, first, max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]), st);
-  const float mc = exponent_base(c, st);
+  move_max<D>(o_addr, c, first, mn, st);
+  const float mc = -c * st.m;
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     uint32_t(&s)[32] = v[q & 1];
@@ -306,10 +336,11 @@ Y2_DEV void softmax_tile(uint32_t s_addr, uint32_t o_addr, float c, bool first, 
     store16(s_addr + 16 * q, p);
     if (q == 2) part();
   }
+  return true;
 }
 
-// The same where rows do not see every key (bit i of `vis`) or the scale is negative. Once or twice
-// a unit; UNROLL 1 keeps it small, as its instructions come from far away (tree attention:
+// The same where rows do not see every key (bit i of `vis`), the scale is negative, or the others
+// turned a tile down. UNROLL 1 keeps it small, as its instructions come from far away (tree attention:
 // full trees 65.4 -> 62.6 us; packed attention is as fast with 4).
 // Masked keys need exact zeros, so no weight is a polynomial's.
 template <int D, bool F16, int UNROLL, class Part>
@@ -337,7 +368,7 @@ Y2_DEV void softmax_masked(uint32_t s_addr, uint32_t o_addr, float c, bool negat
     }
   }
   move_max<D>(o_addr, c, first, max3(mx, my, my), st);
-  const float mc = exponent_base(c, st);
+  const Exponent e(c, st.m);
 #pragma unroll UNROLL
   for (int q = 0; q < 4; ++q) {
     uint32_t p[16];
@@ -349,7 +380,8 @@ Y2_DEV void softmax_masked(uint32_t s_addr, uint32_t o_addr, float c, bool negat
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         float a, b;
-        fma2(a, b, __uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]), c, c, mc, mc);
+        fma2(a, b, __uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]), e.a, e.a, e.b, e.b);
+        mul2(a, b, e.k);
         a = ex2(a);
         b = ex2(b);
         add2(st.l[2 * (i & 1)], st.l[2 * (i & 1) + 1], a, b);
@@ -364,14 +396,14 @@ Y2_DEV void softmax_masked(uint32_t s_addr, uint32_t o_addr, float c, bool negat
 // The same for a tile that every row sees whole, with a positive scale, after the first one: the
 // weights are formed relative to the m there is, the maximum is found on the way, and only
 // when it asks for another m (false: nothing has been written) softmax_masked does the tile.
-// The vote also turns down an m without a finite c m: after tiles without any weight (scores of
-// -inf) m is -inf, which no weight can be taken relative to.
+// The vote also turns down an m out of range: after tiles without any weight (scores of -inf) m is
+// -inf, which no weight can be taken relative to.
 // Without the first pass the exponentials start as soon as the scores are there (8,192 rows of
 // 24 heads, all seen: 756 -> 716 us). Only long packed sequences gain: in tree attention
 // the larger code costs more than the pass (full trees 65.2 -> 67.8 us).
 template <int D, bool F16, class Part>
 Y2_DEV bool softmax_settled(uint32_t s_addr, float c, RowStats& st, Part part) {
-  const float cm = -st.m * c, mc = fabsf(cm) < INFINITY ? cm : NAN;
+  const float mc = in_range(c, st.m) ? -c * st.m : NAN;
   uint32_t v[2][32], p[3][16];
   float l[4] = {0.f, 0.f, 0.f, 0.f}, mx = -INFINITY, my = -INFINITY;
   auto weights = [&](float a, float b, int i, float (&sum)[4]) {
@@ -410,7 +442,7 @@ Y2_DEV bool softmax_settled(uint32_t s_addr, float c, RowStats& st, Part part) {
     if (i & 1) mx = max3(mx, x[2 * i], x[2 * i + 1]);
     else my = max3(my, x[2 * i], x[2 * i + 1]);
   }
-  if (__any_sync(0xffffffffu, !(max3(mx, my, my) <= 8.0f))) return false;
+  if (__any_sync(0xffffffffu, st.live && !(max3(mx, my, my) <= 8.0f))) return false;
 #pragma unroll
   for (int i = 0; i < 4; ++i) st.l[i] += l[i];
 #pragma unroll
@@ -515,6 +547,12 @@ Y2_DEV void add_nonfinite(const uint16_t* v, float (&o)[32]) {
 }
 
 // ---- host
+// c of the exponents. Not below the smallest normal number: a masked score is -inf, and 0 * -inf is
+// not 0. Not above a quarter of the largest: differences of scores are taken in quarters, and
+// with a c like that only the largest score has a weight anyway.
+inline float weight_scale(float scale) {
+  return std::min(std::max(std::fabs(scale) * 1.4426950408889634f, 1.17549435e-38f), 8.5e37f);
+}
 // Tensor map of 16-bit values [.., dims[1], dims[0]] (strides in bytes of the outer
 // dimensions) in boxes of 64 x box1 x box2 values, 128-byte swizzle, zeros beyond the end. The
 // driver's encoder is looked up through the runtime, so that the library loads without a driver.
