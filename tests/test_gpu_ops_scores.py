@@ -235,3 +235,50 @@ def test_packed_one_score_far_above_all_others(ops, scale):
     ops.check_status()
     assert torch.equal(got[at:], v[at].expand(n - at, 2, 128))
     assert torch.isfinite(got[:at]).all()
+
+
+def small_weights(n, dim):
+    """One key far above n - 1 equal ones, 25.5 bits lower, which hold all that some columns get."""
+    q, k = torch.zeros((n, 1, dim), dtype=torch.float16, device=DEV), torch.zeros((n, 1, dim), dtype=torch.float16, device=DEV)
+    q[..., C], k[0, 0, C] = 4, 25.5 * math.log(2) * math.sqrt(dim) / 4
+    v = 1 + randn((n, 1, dim), torch.float16, 3).abs()
+    v[0, :, dim // 2:] = 0
+    return q, k, v
+
+
+def small_tolerance(q, k, v):
+    # half a step for the output and for each weight, the f32 terms of test_gpu_ops, and for weights below
+    # the normal range, which are kept 2^7 times larger than they are, 2^-32 of the largest one each;
+    # an output below the normal range is off by 2^-25
+    dim, scale = q.shape[-1], 1 / math.sqrt(q.shape[-1])
+    s = q[:, 0].double() @ k[:, 0].double().T * scale
+    p = torch.softmax(s, 1)
+    out, size = p @ v[:, 0].double(), p @ v[:, 0].double().abs()
+    delta = (dim + 4) * 2.0 ** -24 * scale * (q[:, 0].double().abs() @ k[:, 0].double().abs().T).amax(1, keepdim=True)
+    tol = 2.0 ** -11 * out.abs() + (2.0 ** -11 + 2 * delta + 2.0 ** -20) * size
+    return out, tol + 2.0 ** -32 * v[:, 0].double().abs().sum(0)[None] + 2.0 ** -25
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_packed_small_weights_in_half_precision(ops, dim):
+    q, k, v = small_weights(2900, dim)
+    got = ops.attention_packed(q, k, v, offsets([2900]), causal=False)
+    want, tol = small_tolerance(q, k, v)
+    close(got[:, 0], want, tol)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("rows", [1, 40])
+def test_tree_small_weights_in_half_precision(ops, rows, dim):
+    n = 6000
+    q, k, v = small_weights(n, dim)
+    pages, table = make_pages(random.Random(3), [n])
+    data = torch.zeros((pages, 1, 2, 1, 64, dim), dtype=torch.float16, device=DEV)
+    pos = torch.arange(n, device=DEV)
+    page = ints(table[0]).long()[pos // 64]
+    data[page, 0, 0, 0, pos % 64], data[page, 0, 1, 0, pos % 64] = k[:, 0], v[:, 0]
+    mask = ints(np.full(rows, -1, dtype=np.int64), torch.int64)  # every row sees every drafted one
+    got = ops.attention_tree(q[:rows], ops.KvPool(data), 0, ints(table), ints([n - rows]), offsets([rows]), mask=mask)
+    ops.check_status()
+    want, tol = small_tolerance(q[:rows], k, v)
+    close(got[:, 0], want, tol)

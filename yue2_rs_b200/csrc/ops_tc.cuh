@@ -188,14 +188,6 @@ Y2_DEV void add2(float& x, float& y, float a, float b) {
       : "f"(a), "f"(b));
 }
 
-Y2_DEV void mul2(float& x, float& y, float a) {
-  asm("{\n\t.reg .b64 s, t;\n\t"
-      "mov.b64 s, {%0, %1};\n\tmov.b64 t, {%2, %2};\n\t"
-      "mul.rn.f32x2 s, s, t;\n\tmov.b64 {%0, %1}, s;\n\t}"
-      : "+f"(x), "+f"(y)
-      : "f"(a));
-}
-
 // The largest of three, NaN if one of them is.
 Y2_DEV float max3(float a, float b, float c) {
   float d;
@@ -262,12 +254,18 @@ Y2_DEV void move_max(uint32_t o_addr, float c, bool first, float mn, RowStats& s
   }
   if (move) st.m = mn;
 }
+
+// Exponents of f16 weights are 7 higher: weights reach 2^8 (move_max), so 2^15 at most, and those down
+// to 2^-21 of the reference instead of 2^-14 are normal numbers (of several thousand keys, each
+// 2^-25 of the largest, nothing was left). The division by l removes it. bf16 has f32's range.
+template <bool F16>
+constexpr float kLift = F16 ? 7.f : 0.f;
 // Whether c s - c m, one FMA, is the exponent of a score s. c m is rounded, so that all weights of the
 // row share a factor of up to 2^(c m 2^-24), which the division by l removes as long as it fits the
 // weights' type: below 2^20 it is at most 2^(1/16). An infinite or NaN m is out of range, too.
 Y2_DEV bool in_range(float c, float m) { return fabsf(c * m) < 0x1p20f; }
-// The exponent of any row: (a s + b) k. An m of +inf or NaN makes the row NaN; an m of -inf (no score
-// above it yet) gives every weight 0.
+// The exponent of any row: (a s + b) k + kLift. An m of +inf or NaN makes the row NaN; an m of -inf
+// (no score above it yet) gives every weight 0.
 struct Exponent {
   float a, b, k;
   Y2_DEV Exponent(float c, float m) {
@@ -283,8 +281,8 @@ struct Exponent {
 // The maximum first (m starts as the first tile's), then the weights in a second pass over the
 // scores in TMEM (reading them again costs less than holding 128 registers). False, and nothing
 // done, when a row's maximum is out of range: softmax_masked does the tile. p is rounded
-// to 16 bits (relative error of half a step, as the output's own rounding; l sums the
-// unrounded weights). kPoly of 16 pairs take the FMA units, the others the special-function
+// to 16 bits (relative error of half a step, as the output's own rounding, and for f16 the range
+// of kLift; l sums the unrounded weights). kPoly of 16 pairs take the FMA units, the others the special-function
 // unit, which alone would need as long as the tensor cores (8,192 rows of 24 heads: 719 us
 // with 0, 712 with 1, 711 with 2, 729 with 4, 767 with 8, where the additional instructions cost
 // more). part() runs when 96 weights are stored; the caller announces the last 32.
@@ -312,7 +310,7 @@ Y2_DEV bool softmax_tile(uint32_t s_addr, uint32_t o_addr, float c, bool first, 
   if (__any_sync(0xffffffffu, st.live && !in_range(c, mn))) return false;
   load32(s_addr, v[0]);
   move_max<D>(o_addr, c, first, mn, st);
-  const float mc = -c * st.m;
+  const float mc = fmaf(-c, st.m, kLift<F16>);
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     uint32_t(&s)[32] = v[q & 1];
@@ -381,7 +379,7 @@ Y2_DEV void softmax_masked(uint32_t s_addr, uint32_t o_addr, float c, bool negat
       for (int i = 0; i < 16; ++i) {
         float a, b;
         fma2(a, b, __uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]), e.a, e.a, e.b, e.b);
-        mul2(a, b, e.k);
+        fma2(a, b, a, b, e.k, e.k, kLift<F16>, kLift<F16>);
         a = ex2(a);
         b = ex2(b);
         add2(st.l[2 * (i & 1)], st.l[2 * (i & 1) + 1], a, b);
@@ -403,7 +401,7 @@ Y2_DEV void softmax_masked(uint32_t s_addr, uint32_t o_addr, float c, bool negat
 // the larger code costs more than the pass (full trees 65.2 -> 67.8 us).
 template <int D, bool F16, class Part>
 Y2_DEV bool softmax_settled(uint32_t s_addr, float c, RowStats& st, Part part) {
-  const float mc = in_range(c, st.m) ? -c * st.m : NAN;
+  const float mc = in_range(c, st.m) ? fmaf(-c, st.m, kLift<F16>) : NAN;
   uint32_t v[2][32], p[3][16];
   float l[4] = {0.f, 0.f, 0.f, 0.f}, mx = -INFINITY, my = -INFINITY;
   auto weights = [&](float a, float b, int i, float (&sum)[4]) {
@@ -442,7 +440,7 @@ Y2_DEV bool softmax_settled(uint32_t s_addr, float c, RowStats& st, Part part) {
     if (i & 1) mx = max3(mx, x[2 * i], x[2 * i + 1]);
     else my = max3(my, x[2 * i], x[2 * i + 1]);
   }
-  if (__any_sync(0xffffffffu, st.live && !(max3(mx, my, my) <= 8.0f))) return false;
+  if (__any_sync(0xffffffffu, st.live && !(max3(mx, my, my) <= 8.0f + kLift<F16>))) return false;
 #pragma unroll
   for (int i = 0; i < 4; ++i) st.l[i] += l[i];
 #pragma unroll
