@@ -6,8 +6,8 @@ Every call runs on the current stream of its tensors' device, allocates through 
 (outputs and workspaces) and can be captured into a CUDA graph: lengths, page tables and
 lists are read on the device. Sizes, types and strides are checked at once (Yue2Error); what
 only the device sees (page indexes, lengths, positions) is checked there, an entry out of
-range is skipped, and `check_status` reports it. The operators serve: they have no backward
-pass, and refuse rows that ask for one.
+range is skipped, and `check_status` reports it. The operators serve: they have no gradients,
+and refuse rows, gains, tables and pools that ask for one.
 
 A step over a batch of requests: `qk_rope_append` writes the new rows' K and V into the pages,
 `attention_packed` attends over whole prompts, `attention_tree` checks drafted tokens against
@@ -18,6 +18,7 @@ import ctypes
 import threading
 
 import torch
+from torch.autograd import forward_ad as _forward  # its _current_level: -1 outside of any dual level
 
 from . import _lib
 
@@ -123,6 +124,12 @@ def _no_gradient(what):
         raise _invalid(f"{what} asks for a gradient, which these operators do not have: call them under torch.no_grad()")
 
 
+def _no_tangents(*tensors):
+    for t in tensors:
+        if t is not None and _forward.unpack_dual(t).tangent is not None:
+            raise _invalid("a tensor carries a tangent, and these operators have no forward-mode gradient")
+
+
 def _rows(t, index, dtype, what, shape=None):
     """The address, row stride and shape of a [rows, heads, dim] tensor with adjacent heads."""
     if t.dtype is not dtype or t.get_device() != index or t.dim() != 3 or (shape is not None and t.shape != shape):
@@ -169,6 +176,8 @@ def qk_rope_append(qkv, q_norm, k_norm, eps, cos, sin, positions, pool, layer, s
     K as well. q_out and k_out may be the q and k parts of qkv."""
     dev, dtype, kv, f32 = pool.index, pool.dtype, pool.kv_heads, torch.float32
     src, stride, rows, width, dim = _rows(qkv, dev, dtype, "qkv")
+    if pool.data.requires_grad:
+        _no_gradient("the pool")
     heads = width - 2 * kv
     if heads < 1 or dim != pool.dim:
         raise _invalid("qkv must be [rows, heads + 2 kv heads, dim] of the pool's kv heads and dim")
@@ -179,6 +188,10 @@ def qk_rope_append(qkv, q_norm, k_norm, eps, cos, sin, positions, pool, layer, s
         raise _invalid("q_norm and k_norm go together")
     if q_norm is not None and (q_norm.requires_grad or k_norm.requires_grad):
         _no_gradient("the norm")
+    if cos.requires_grad or sin.requires_grad:
+        _no_gradient("the table of cos or sin")
+    if _forward._current_level >= 0:
+        _no_tangents(qkv, q_norm, k_norm, cos, sin, pool.data, q_out, k_out)
     if q_out is None:
         q_out = qkv.new_empty((rows, heads, dim))
         qp, qs = q_out.data_ptr(), heads * dim
@@ -205,6 +218,8 @@ def attention_packed(q, k, v, cu, causal=True, scale=None, out=None):
     code = _DTYPES.get(dtype)
     if code is None or dev < 0:
         raise _invalid("attention takes bf16 or f16 tensors on a GPU")
+    if _forward._current_level >= 0:
+        _no_tangents(q, k, v, out)
     qp, qs, tokens, heads, dim = _rows(q, dev, dtype, "q")
     kp, ks, keys, kv, kdim = _rows(k, dev, dtype, "k")
     vp, vs = _rows(v, dev, dtype, "v", (tokens, kv, dim))[:2]
@@ -233,9 +248,13 @@ def attention_tree(q, pool, layer, table, context, cu, mask=None, scale=None, ou
     zeros; rows outside [cu[0], cu[-1]) of `out` are left as they were (undefined when `out` is
     None)."""
     dev, dtype, i32 = pool.index, pool.dtype, torch.int32
+    if pool.data.requires_grad:
+        _no_gradient("the pool")
     qp, qs, rows, heads, dim = _rows(q, dev, dtype, "q")
     if dim != pool.dim:
         raise _invalid("q must have the pool's dim")
+    if _forward._current_level >= 0:
+        _no_tangents(q, pool.data, out)
     if out is None:
         out = q.new_empty((rows, heads, dim))
         op, os_ = out.data_ptr(), heads * dim
@@ -255,6 +274,10 @@ def kv_copy(pool, src, dst, count=None):
     """Positions [0, count[i]) (all 64 when count is None) of page src[i] to page dst[i], in
     every layer; int32 [n] each. The dst pages are distinct and none of them is a src page."""
     dev, i32, n = pool.index, torch.int32, src.shape[0]
+    if pool.data.requires_grad:
+        _no_gradient("the pool")
+    if _forward._current_level >= 0:
+        _no_tangents(pool.data)
     _call(dev, "yue2_kv_copy", pool._ref, _flat(src, i32, dev, "src", n), _flat(dst, i32, dev, "dst", n),
           0 if count is None else _flat(count, i32, dev, "count", n), n)
 
@@ -267,12 +290,16 @@ def kv_gather(pool, src_table, dst_table, begin, cu, keep):
     own. Otherwise into the pages of dst_table, none of which the call reads; keep in any
     order. Tables int32 [seqs, pages], begin int32 [seqs], cu int32 [seqs + 1], keep int32."""
     dev, i32 = pool.index, torch.int32
+    if pool.data.requires_grad:
+        _no_gradient("the pool")
     sp, seqs, pages = _table(src_table, i32, dev, "src_table")
     dp, dst_seqs, dst_pages = (0, seqs, 0) if dst_table is None else _table(dst_table, i32, dev, "dst_table")
     if dst_seqs != seqs:
         raise _invalid("src_table and dst_table must hold the same sequences")
     if keep.dim() != 1:
         raise _invalid("keep must be one list")
+    if _forward._current_level >= 0:
+        _no_tangents(pool.data)
     total = keep.shape[0]
     _call(dev, "yue2_kv_gather", pool._ref, sp, pages, dp, dst_pages, _flat(begin, i32, dev, "begin", seqs),
           _flat(cu, i32, dev, "cu", seqs + 1), _flat(keep, i32, dev, "keep", total), seqs, total)
