@@ -67,3 +67,32 @@ def test_tangents_are_refused(ops, which):
                 ops.qk_rope_append(dual(qkv, "qkv"), dual(gain, "gain"), gain, 1e-6, dual(cos, "cos"), sin, pos, ops.KvPool(data), 0, slots)
         ops.attention_packed(q, k, k, cu)  # tensors without a tangent are taken at this level too
     ops.check_status()
+
+
+def test_what_is_written_counts_as_modified(ops):
+    # a product that saved the buffer for its backward pass must not use what is there later
+    q, k = randn((10, 4, 64), torch.bfloat16, 1), randn((10, 2, 64), torch.bfloat16, 2)
+    cu, table = offsets([10]), ints([[0, 1]])
+    qkv, cos, sin, pos, slots = append_args()
+    writes = {
+        "packed": lambda b, p: ops.attention_packed(q, k, k, cu, out=b),
+        "tree": lambda b, p: ops.attention_tree(q, p, 0, table, ints([0]), cu, out=b),
+        "q_out": lambda b, p: ops.qk_rope_append(qkv, None, None, 0.0, cos, sin, pos, p, 0, slots, q_out=b),
+        "k_out": lambda b, p: ops.qk_rope_append(qkv, None, None, 0.0, cos, sin, pos, p, 0, slots, k_out=b[:, :2])}
+    for name, write in writes.items():
+        b = randn((10, 4, 64), torch.bfloat16, 5)
+        w = torch.ones_like(b, requires_grad=True)
+        y = (w * b).sum()
+        write(b, ops.KvPool(randn((2, 1, 2, 2, 64, 64), torch.bfloat16, 3)))
+        with pytest.raises(RuntimeError, match="modified by an inplace"):
+            y.backward()
+            pytest.fail(f"{name} went unnoticed")
+    for name in ("append", "copy", "gather"):
+        data = randn((2, 1, 2, 2, 64, 64), torch.bfloat16, 3)
+        w = torch.ones_like(data, requires_grad=True)
+        y = (w * data).sum()
+        calls(ops, data)[name]()
+        with pytest.raises(RuntimeError, match="modified by an inplace"):
+            y.backward()
+            pytest.fail(f"{name} went unnoticed")
+    ops.check_status()

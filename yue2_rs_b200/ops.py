@@ -105,6 +105,11 @@ class KvPool:
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
 
 
+# What the kernels write through an address counts as modified in place, so that a backward pass which
+# saved it notices.
+_written = torch.autograd.graph.increment_version
+
+
 def _flat(t, dtype, index, what, count):
     """The address of a contiguous device tensor of `count` values."""
     if t.dtype is dtype and t.get_device() == index and t.numel() == count and t.is_contiguous():
@@ -203,6 +208,7 @@ def qk_rope_append(qkv, q_norm, k_norm, eps, cos, sin, positions, pool, layer, s
           0 if k_norm is None else _flat(k_norm, f32, dev, "k_norm", dim), eps, cp, _flat(sin, f32, dev, "sin", steps * half), steps,
           _flat(positions, torch.int32, dev, "positions", rows), pool._ref, layer, _flat(slots, torch.int64, dev, "slots", rows),
           qp, qs, kp if rows else 0, ks)
+    _written((q_out, pool.data) if k_out is None else (q_out, pool.data, k_out))
     return q_out
 
 
@@ -235,6 +241,7 @@ def attention_packed(q, k, v, cu, causal=True, scale=None, out=None):
     seqs = cu.shape[0] - 1
     _call(dev, "yue2_attention_packed", qp, kp, vp, op, _flat(cu, torch.int32, dev, "cu", seqs + 1), seqs, tokens,
           heads, kv, dim, qs, ks, vs, os_, code, 1 if causal else 0, dim ** -0.5 if scale is None else scale)
+    _written(out)
     return out
 
 
@@ -267,6 +274,7 @@ def attention_tree(q, pool, layer, table, context, cu, mask=None, scale=None, ou
           _flat(context, i32, dev, "context", seqs), _flat(cu, i32, dev, "cu", seqs + 1),
           0 if mask is None else _flat(mask, torch.int64, dev, "mask", rows), dim ** -0.5 if scale is None else scale,
           op, os_, work.data_ptr() if need else 0, need)
+    _written(out)
     return out
 
 
@@ -280,6 +288,7 @@ def kv_copy(pool, src, dst, count=None):
         _no_tangents(pool.data)
     _call(dev, "yue2_kv_copy", pool._ref, _flat(src, i32, dev, "src", n), _flat(dst, i32, dev, "dst", n),
           0 if count is None else _flat(count, i32, dev, "count", n), n)
+    _written(pool.data)
 
 
 def kv_gather(pool, src_table, dst_table, begin, cu, keep):
@@ -303,3 +312,4 @@ def kv_gather(pool, src_table, dst_table, begin, cu, keep):
     total = keep.shape[0]
     _call(dev, "yue2_kv_gather", pool._ref, sp, pages, dp, dst_pages, _flat(begin, i32, dev, "begin", seqs),
           _flat(cu, i32, dev, "cu", seqs + 1), _flat(keep, i32, dev, "keep", total), seqs, total)
+    _written(pool.data)
