@@ -96,3 +96,18 @@ def test_what_is_written_counts_as_modified(ops):
             y.backward()
             pytest.fail(f"{name} went unnoticed")
     ops.check_status()
+
+
+def test_a_first_call_in_inference_mode_reports_as_any(ops, monkeypatch):
+    monkeypatch.setattr(ops, "_status", {})
+    data = randn((2, 1, 2, 1, 64, 64), torch.bfloat16, 1)
+    with torch.inference_mode():
+        ops.kv_copy(ops.KvPool(data), ints([0]), ints([7]))
+    with pytest.raises(Yue2Error, match="page index"):
+        ops.check_status()
+    ops.check_status()  # cleared
+    with torch.inference_mode():
+        ops.kv_copy(ops.KvPool(torch.zeros_like(data)), ints([-1]), ints([1]))
+        with pytest.raises(Yue2Error, match="page index"):
+            ops.check_status()
+        ops.check_status()

@@ -46,7 +46,8 @@ def _status_of(index):
                 raise _invalid("call an operator (or check_status) once on this device before any capture")
             s = _status.get(index)
             if s is None:
-                word = torch.zeros(1, dtype=torch.int32, device=device)
+                with torch.inference_mode(False):  # check_status clears it in either mode
+                    word = torch.zeros(1, dtype=torch.int32, device=device)
                 torch.cuda.synchronize(device)  # cleared before any stream's kernels see it
                 s = _status[index] = (word.data_ptr(), word)
     return s[0]
