@@ -111,3 +111,19 @@ def test_a_first_call_in_inference_mode_reports_as_any(ops, monkeypatch):
         with pytest.raises(Yue2Error, match="page index"):
             ops.check_status()
         ops.check_status()
+
+
+def test_a_check_inside_a_capture_is_refused_and_the_capture_lives(ops):
+    data = randn((2, 1, 2, 1, 64, 64), torch.bfloat16, 1)
+    pool, src, dst = ops.KvPool(data), ints([0]), ints([1])
+    ops.kv_copy(pool, src, dst)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(Yue2Error, match="capture"):
+            ops.check_status()
+        ops.kv_copy(pool, src, dst)
+    data[0] = 3
+    graph.replay()
+    ops.check_status()
+    assert (data[1] == 3).all()

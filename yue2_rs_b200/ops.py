@@ -55,7 +55,9 @@ def _status_of(index):
 
 def check_status(device=None):
     """Waits for the device, then raises Yue2Error for what the operators' kernels found since
-    the last check and clears it."""
+    the last check and clears it. Not for use inside a capture, which no wait survives."""
+    if torch.cuda.is_current_stream_capturing():
+        raise _invalid("check_status waits for the device: call it outside of a capture")
     device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     if device.index is None:
         device = torch.device("cuda", torch.cuda.current_device())
