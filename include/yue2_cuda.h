@@ -366,7 +366,8 @@ int yue2_bench_gemv(Yue2Model* m, int kind, int rows, int launches, double* avg_
  * that the caller clears and reads when it likes.
  *
  * Vectors of one head are contiguous and the heads of a row adjacent; row strides are in
- * elements, a multiple of 8, and every base is 16-byte aligned. Values are bf16 or f16. */
+ * elements, a multiple of 8, and every base is 16-byte aligned. Values are bf16 or f16. Lists,
+ * tables and masks are aligned to their entries. */
 #define YUE2_STATUS_PAGE 1  /* a page index or slot outside the pool */
 #define YUE2_STATUS_RANGE 2 /* a length, offset or position outside its buffer or table */
 #define YUE2_STATUS_STALL 4 /* a bounded device wait gave up: the call's outputs are invalid */

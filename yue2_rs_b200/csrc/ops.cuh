@@ -94,6 +94,13 @@ inline int check_rows(const void* p, uint64_t rows, uint64_t heads, uint64_t dim
   return 0;
 }
 
+// A list of `size`-byte entries (NULL passes: who needs one looks for it first).
+inline int check_list(const void* p, size_t size, const char* what) {
+  if ((uintptr_t)p & (size - 1))
+    return fail(YUE2_ERR_INVALID, std::string(what) + " must be aligned to its " + std::to_string(size) + "-byte entries");
+  return 0;
+}
+
 inline int check_heads(uint64_t heads, uint64_t kv) {
   if (heads == 0 || kv == 0 || heads > 1024 || kv > 1024 || heads % kv)
     return fail(YUE2_ERR_INVALID, "heads must be a multiple of kv, both in [1, 1024]");

@@ -445,6 +445,7 @@ extern "C" int yue2_attention_packed(const void* q, const void* k, const void* v
     return rc;
   if (seqs == 0 || tokens == 0) return 0;
   if (!cu) return fail(YUE2_ERR_INVALID, "null sequence offsets");
+  if ((rc = check_list(cu, 4, "cu"))) return rc;
   const bool f16 = dtype == YUE2_DTYPE_F16;
   CUtensorMap mq, mk, mv;
   if (!opt::make_rows_map(&mq, f16, q, tokens, heads, dim, q_stride, 1, opt::kRows) ||

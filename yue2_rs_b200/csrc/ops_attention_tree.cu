@@ -720,6 +720,9 @@ int yue2_attention_tree(const void* q, uint64_t rows, uint64_t heads, uint64_t q
     return rc;
   if (seqs == 0 || rows == 0) return 0;
   if (!table || !context || !cu) return fail(YUE2_ERR_INVALID, "null page table, context or row offsets");
+  if ((rc = check_list(table, 4, "table")) || (rc = check_list(context, 4, "context")) || (rc = check_list(cu, 4, "cu")) ||
+      (rc = check_list(mask, 8, "mask")))
+    return rc;
   const uint64_t pool_rows = (uint64_t)v.pages * v.blocks * kPageTokens;
   if (pool_rows > (uint64_t)INT32_MAX) return fail(YUE2_ERR_INVALID, "the KV pool has more than 2^31 head rows");
   int sms = 0;

@@ -277,6 +277,7 @@ int yue2_qk_rope_append(const void* qkv, uint64_t rows, uint64_t heads, uint64_t
     return fail(YUE2_ERR_INVALID, "positions, slots and 16-byte aligned cos and sin tables are needed");
   if (!(eps >= 0.f)) return fail(YUE2_ERR_INVALID, "eps must not be negative");
   if (rows == 0) return 0;
+  if ((rc = check_list(positions, 4, "positions")) || (rc = check_list(slots, 8, "slots"))) return rc;
   p.qkv = (const uint16_t*)qkv;
   p.q_out = (uint16_t*)q_out;
   p.k_out = (uint16_t*)k_out;
@@ -319,6 +320,7 @@ int yue2_kv_copy(const Yue2KvPool* pool, const int32_t* src, const int32_t* dst,
   if (n > 65535) return fail(YUE2_ERR_INVALID, "at most 65,535 page pairs per call");
   if (n && (!src || !dst)) return fail(YUE2_ERR_INVALID, "null page list");
   if (n == 0) return 0;
+  if ((rc = check_list(src, 4, "src")) || (rc = check_list(dst, 4, "dst")) || (rc = check_list(count, 4, "count"))) return rc;
   kv_copy_kernel<<<dim3((unsigned)v.blocks, (unsigned)n), kMoveThreads, 0, static_cast<cudaStream_t>(stream)>>>(
       v, src, dst, count, status);
   const cudaError_t e = cudaGetLastError();
@@ -335,6 +337,9 @@ int yue2_kv_gather(const Yue2KvPool* pool, const int32_t* src_table, uint64_t sr
     return fail(YUE2_ERR_INVALID, "at most 65,535 sequences, 2^31 - 1 list entries and 2^26 pages per table row");
   if (seqs == 0 || total == 0) return 0;
   if (!src_table || !begin || !cu || !keep) return fail(YUE2_ERR_INVALID, "null table or list");
+  if ((rc = check_list(src_table, 4, "src_table")) || (rc = check_list(dst_table, 4, "dst_table")) ||
+      (rc = check_list(begin, 4, "begin")) || (rc = check_list(cu, 4, "cu")) || (rc = check_list(keep, 4, "keep")))
+    return rc;
   p.src_table = src_table;
   p.dst_table = dst_table;
   p.begin = begin;
