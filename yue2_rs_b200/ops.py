@@ -66,7 +66,7 @@ def check_status(device=None):
     torch.cuda.synchronize(device)
     bits = int(s.item())
     if bits:
-        s.zero_()
+        s.bitwise_and_(~bits)  # not what other threads' calls have found since
         torch.cuda.synchronize(device)
         text = "; ".join(t for b, t in _BITS if bits & b)
         raise _lib.Yue2Error(-7 if bits & 4 else -1, text)
