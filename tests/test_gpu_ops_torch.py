@@ -127,3 +127,12 @@ def test_a_check_inside_a_capture_is_refused_and_the_capture_lives(ops):
     graph.replay()
     ops.check_status()
     assert (data[1] == 3).all()
+
+
+def test_odd_arguments_raise_the_wrappers_error(ops):
+    pool = ops.KvPool(randn((2, 1, 2, 2, 64, 64), torch.bfloat16, 3))
+    empty = torch.empty((4, 2, 0), dtype=torch.bfloat16, device=DEV)
+    for f in (lambda: ops.attention_packed(empty, empty, empty, offsets([4])),
+              lambda: ops.kv_copy(pool, torch.tensor(0, dtype=torch.int32, device=DEV), torch.tensor(1, dtype=torch.int32, device=DEV))):
+        with pytest.raises(Yue2Error):
+            f()

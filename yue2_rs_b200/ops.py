@@ -243,7 +243,7 @@ def attention_packed(q, k, v, cu, causal=True, scale=None, out=None):
         raise _invalid("cu must be [seqs + 1]")
     seqs = cu.shape[0] - 1
     _call(dev, "yue2_attention_packed", qp, kp, vp, op, _flat(cu, torch.int32, dev, "cu", seqs + 1), seqs, tokens,
-          heads, kv, dim, qs, ks, vs, os_, code, 1 if causal else 0, dim ** -0.5 if scale is None else scale)
+          heads, kv, dim, qs, ks, vs, os_, code, 1 if causal else 0, (dim or 1) ** -0.5 if scale is None else scale)
     _written(out)
     return out
 
@@ -275,7 +275,7 @@ def attention_tree(q, pool, layer, table, context, cu, mask=None, scale=None, ou
     work = q.new_empty((need + 1) // 2) if need else None  # 16-bit values
     _call(dev, "yue2_attention_tree", qp, rows, heads, qs, pool._ref, layer, tp, seqs, pages,
           _flat(context, i32, dev, "context", seqs), _flat(cu, i32, dev, "cu", seqs + 1),
-          0 if mask is None else _flat(mask, torch.int64, dev, "mask", rows), dim ** -0.5 if scale is None else scale,
+          0 if mask is None else _flat(mask, torch.int64, dev, "mask", rows), (dim or 1) ** -0.5 if scale is None else scale,
           op, os_, work.data_ptr() if need else 0, need)
     _written(out)
     return out
@@ -284,6 +284,8 @@ def attention_tree(q, pool, layer, table, context, cu, mask=None, scale=None, ou
 def kv_copy(pool, src, dst, count=None):
     """Positions [0, count[i]) (all 64 when count is None) of page src[i] to page dst[i], in
     every layer; int32 [n] each. The dst pages are distinct and none of them is a src page."""
+    if src.dim() != 1:
+        raise _invalid("src must be one list")
     dev, i32, n = pool.index, torch.int32, src.shape[0]
     if pool.data.requires_grad:
         _no_gradient("the pool")
