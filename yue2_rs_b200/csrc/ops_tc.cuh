@@ -277,16 +277,17 @@ struct Exponent {
 };
 
 // A side's softmax over one tile of 128 keys: the scores in TMEM become weights
-// p = 2^(c (s - m)), packed over them. c = |scale| log2(e), weight_scale. Every lane of the warp takes part.
-// The maximum first (m starts as the first tile's), then the weights in a second pass over the
-// scores in TMEM (reading them again costs less than holding 128 registers). False, and nothing
-// done, when a row's maximum is out of range: softmax_masked does the tile. p is rounded
-// to 16 bits (relative error of half a step, as the output's own rounding, and for f16 the range
-// of kLift; l sums the unrounded weights). kPoly of 16 pairs take the FMA units, the others the special-function
-// unit, which alone would need as long as the tensor cores (8,192 rows of 24 heads: 719 us
-// with 0, 712 with 1, 711 with 2, 729 with 4, 767 with 8, where the additional instructions cost
-// more). part() runs when 96 weights are stored; the caller announces the last 32.
-constexpr int kPoly = 2;
+// p = 2^(c (s - m)), packed over them. c = |scale| log2(e), see weight_scale. Every lane of the
+// warp takes part. The maximum first (m starts as the first tile's), then the weights in a second
+// pass over the scores in TMEM (reading them again costs less than holding 128 registers). False,
+// and nothing done, when a row's maximum is out of range: softmax_masked does the tile. p is
+// rounded to 16 bits (relative error of half a step, as the output's own rounding, and for f16 the
+// range of kLift; l sums the unrounded weights). kPoly of 16 pairs take the FMA units, the others
+// the special-function unit (trees, captured, with 0 / 1 / 2 / 4 of 16: full trees 65.4 / 60.0 /
+// 63.9 / 59.1 us, a batch 44.9 / 42.5 / 45.0 / 42.3). In packed attention's softmax_settled they gain
+// nothing: 8,192 rows of 24 heads 760 us with none and 773 with 2, prompt pair 30.1 and 29.8.
+// part() runs when 96 weights are stored; the caller announces the last 32.
+constexpr int kPoly = 1;
 template <int D, bool F16, class Part>
 Y2_DEV bool softmax_tile(uint32_t s_addr, uint32_t o_addr, float c, bool first, RowStats& st, Part part) {
   uint32_t v[2][32];
@@ -340,7 +341,6 @@ Y2_DEV bool softmax_tile(uint32_t s_addr, uint32_t o_addr, float c, bool first, 
 // The same where rows do not see every key (bit i of `vis`), the scale is negative, or the others
 // turned a tile down. UNROLL 1 keeps it small, as its instructions come from far away (tree attention:
 // full trees 65.4 -> 62.6 us; packed attention is as fast with 4).
-// Masked keys need exact zeros, so no weight is a polynomial's.
 template <int D, bool F16, int UNROLL, class Part>
 Y2_DEV void softmax_masked(uint32_t s_addr, uint32_t o_addr, float c, bool negate, bool first, const uint32_t (&vis)[4],
                            RowStats& st, Part part) {
@@ -397,20 +397,16 @@ Y2_DEV void softmax_masked(uint32_t s_addr, uint32_t o_addr, float c, bool negat
 // The vote also turns down an m out of range: after tiles without any weight (scores of -inf) m is
 // -inf, which no weight can be taken relative to.
 // Without the first pass the exponentials start as soon as the scores are there (8,192 rows of
-// 24 heads, all seen: 756 -> 716 us). Only long packed sequences gain: in tree attention
-// the larger code costs more than the pass (full trees 65.2 -> 67.8 us).
+// 24 heads, all seen, when this form was added: 756 -> 716 us in bursts). Only long packed
+// sequences gain: in tree attention the larger code cost more than the pass (65.2 -> 67.8 us).
 template <int D, bool F16, class Part>
 Y2_DEV bool softmax_settled(uint32_t s_addr, float c, RowStats& st, Part part) {
   const float mc = in_range(c, st.m) ? fmaf(-c, st.m, kLift<F16>) : NAN;
   uint32_t v[2][32], p[3][16];
   float l[4] = {0.f, 0.f, 0.f, 0.f}, mx = -INFINITY, my = -INFINITY;
   auto weights = [&](float a, float b, int i, float (&sum)[4]) {
-    if (i % (16 / kPoly) == 16 / kPoly - 1) {
-      poly_ex2<F16>(a, b);
-    } else {
-      a = ex2(a);
-      b = ex2(b);
-    }
+    a = ex2(a);
+    b = ex2(b);
     add2(sum[2 * (i & 1)], sum[2 * (i & 1) + 1], a, b);
     return pack16<F16>(a, b);
   };
