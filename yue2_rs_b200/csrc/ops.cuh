@@ -50,10 +50,6 @@ Y2_DEV void unpack8(const uint4& w, float (&v)[8]) {
   v[0] = lo16<F16>(w.x), v[1] = hi16<F16>(w.x), v[2] = lo16<F16>(w.y), v[3] = hi16<F16>(w.y);
   v[4] = lo16<F16>(w.z), v[5] = hi16<F16>(w.z), v[6] = lo16<F16>(w.w), v[7] = hi16<F16>(w.w);
 }
-template <bool F16>
-Y2_DEV uint4 pack8(const float (&v)[8]) {
-  return make_uint4(pack16<F16>(v[0], v[1]), pack16<F16>(v[2], v[3]), pack16<F16>(v[4], v[5]), pack16<F16>(v[6], v[7]));
-}
 
 // ---- host checks; each returns 0 or the error of fail()
 inline bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
