@@ -103,6 +103,14 @@ inline int check_heads(uint64_t heads, uint64_t kv) {
   return 0;
 }
 
+// SMs of the current device.
+inline int sm_count(int& sms) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  return e == cudaSuccess ? 0 : cuda_fail(e, "device attributes");
+}
+
 inline int check_scale(float scale) {
   if (!std::isfinite(scale)) return fail(YUE2_ERR_INVALID, "scale must be finite");
   return 0;

@@ -642,13 +642,6 @@ __global__ void __launch_bounds__(kMergeThreads, 6) tree_merge_kernel(const Tree
   for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = pack16<F16>(o[e], o[e + 1]);
 }
 
-int sm_count(int& sms) {
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  return e == cudaSuccess ? 0 : cuda_fail(e, "device attributes");
-}
-
 // Nodes of a side, CTAs and the rows of a partial result.
 struct Plan {
   int nodes, ctas, slot_rows;

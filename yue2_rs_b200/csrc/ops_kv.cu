@@ -7,6 +7,7 @@
 // layers (58 MB) 11.3 us; accepting 8 of 64 nodes of 16 trees (29 MB in runs of 256 bytes)
 // 9.7 us, mostly the chain of list, table and row; evicting 4,001 of 8,192 positions (918 MB)
 // 147 us (6.2 TB/s).
+#include <algorithm>
 #include <string>
 
 #include "ops.cuh"
@@ -34,7 +35,9 @@ struct AppendParams {
   float eps;
 };
 
-constexpr int kAppendThreads = 64;  // 8,192 rows of 40 heads: 40.9 us; 128 threads 45.4, 256 51.3
+// 8,192 rows of 40 heads of 128, captured: 31.4 us with 64 threads, 33.9 with 128, 41.5 with 256 (two rows
+// alone: 3.4, 2.3 and 2.0).
+constexpr int kAppendThreads = 64;
 
 Y2_DEV void load4(const float* p, float (&v)[4]) {
   const float4 a = *reinterpret_cast<const float4*>(p);
@@ -138,6 +141,11 @@ __global__ void __launch_bounds__(kAppendThreads) qk_rope_append_kernel(const Ap
   }
 }
 
+// The heads of a group are loaded together where they are up to three, otherwise five at a time. 8,192
+// rows, captured, with 1 / 2 / 3 / 5 loaded together (8 for the last): one head a group (4 + 4 of 64)
+// 6.3 / 6.5 / 6.9 / 7.7 us, two (4 + 4 of 128) 11.9 / 10.7 / 10.9 / -, three (8 + 4 of 128)
+// 16.0 / 15.2 / 13.4 / 14.4, eight (16 + 16) 35.4 / 30.1 / 28.7 / 27.6 (29.3), ten (24 + 16) 42.4 / 35.5
+// / 34.2 / 31.4 (38.4).
 template <int D, bool F16>
 void launch_append(const AppendParams& p, unsigned rows, cudaStream_t st) {
   constexpr int GROUPS = kAppendThreads / (D / 8);
@@ -350,11 +358,13 @@ int yue2_kv_gather(const Yue2KvPool* pool, const int32_t* src_table, uint64_t sr
   p.dst_pages = (long long)dst_pages;
   p.total = (long long)total;
   // Out of place: a warp group per group of rows of the average list, at most 256 shares. A warp
-  // takes several blocks as long as that leaves about 16 warps for each SM.
+  // takes several blocks, four at most, as long as that leaves about 16 warps for each SM.
+  int sms = 0;
+  if ((rc = sm_count(sms))) return rc;
   const uint64_t rows = 256 / pool->dim * kMoveUnroll;
   const uint64_t shares = dst_table ? std::min<uint64_t>(256, (total / seqs + rows - 1) / rows) : 1;
   const unsigned z = (unsigned)std::max<uint64_t>(1, shares);
-  p.per_warp = (int)std::max<uint64_t>(1, std::min<uint64_t>(4, (uint64_t)p.pool.blocks * seqs * z / 2368));
+  p.per_warp = (int)std::max<uint64_t>(1, std::min<uint64_t>(4, (uint64_t)p.pool.blocks * seqs * z / (16 * (uint64_t)sms)));
   const int per_cta = kMoveThreads / 32 * p.per_warp;
   const dim3 grid((unsigned)((p.pool.blocks + per_cta - 1) / per_cta), (unsigned)seqs, z);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
