@@ -404,7 +404,8 @@ int yue2_qk_rope_append(const void* qkv, uint64_t rows, uint64_t heads, uint64_t
  * A key whose score is -inf has no weight, and a row of such keys alone is zero. Rows of `out`
  * outside [cu[0], cu[seqs]) are left as they were, and what a masked position or a row outside
  * the sequence holds (infinities and NaN included) reaches no output. `out` may be q itself
- * (same base and stride) and overlaps neither k nor v. dim 64 or 128, heads a multiple of kv. */
+ * (same base and stride) and overlaps neither k nor v. dim 64 or 128, heads a multiple of kv.
+ * Scores and the sums before the division are f32: values of up to 2^85 cannot overflow them. */
 int yue2_attention_packed(const void* q, const void* k, const void* v, void* out, const int32_t* cu, uint64_t seqs,
                           uint64_t tokens, uint64_t heads, uint64_t kv, uint64_t dim, uint64_t q_stride,
                           uint64_t k_stride, uint64_t v_stride, uint64_t out_stride, int32_t dtype, int32_t causal,
@@ -418,10 +419,10 @@ int yue2_attention_packed(const void* q, const void* k, const void* v, void* out
  * so T = 1 is an ordinary decode step. A row that sees nothing, or scores of -inf alone, gets
  * zeros; rows of `out` outside [cu[0], cu[seqs]) are left as they were; what a masked or unused
  * place of a page holds reaches no output; a sequence with a bad page index has undefined
- * outputs. `out` does not overlap q. At most 1,024 sequences and 128 query heads per kv head, and a pool of fewer
- * than 2^31 [dim] rows. `workspace`:
- * yue2_attention_tree_workspace bytes (0: may be NULL), 16-byte aligned, contents free before
- * and after; calls that may overlap need their own. */
+ * outputs. `out` does not overlap q. Scores and sums as in yue2_attention_packed. At most 1,024
+ * sequences and 128 query heads per kv head, and a pool of fewer than 2^31 [dim] rows.
+ * `workspace`: yue2_attention_tree_workspace bytes (0: may be NULL), 16-byte aligned, contents
+ * free before and after; calls that may overlap need their own. */
 uint64_t yue2_attention_tree_workspace(uint64_t rows, uint64_t heads, uint64_t seqs, uint64_t table_pages,
                                        const Yue2KvPool* pool);
 int yue2_attention_tree(const void* q, uint64_t rows, uint64_t heads, uint64_t q_stride, const Yue2KvPool* pool,

@@ -13,17 +13,23 @@
 //                   under it;
 //   warp 9          picks the units, publishes them to the others and loads Q and the K, V ring by
 //                   TMA.
-// Units go out longest first (a causal unit's cost grows with its block), dealt to the CTAs
-// there and back (0..G-1, G-1..0, ..), found from the offsets on the device, so the host needs no
-// lengths. Heads of one block are neighbours, so that a group's K and V come from L2.
+// Units go out by block index from the highest down, dealt to the CTAs there and back (0..G-1,
+// G-1..0, ..), found from the offsets on the device, so the host needs no lengths. With the causal
+// mask that is longest first. Without it a unit's cost is its sequence's, so sequences of different
+// lengths are dealt unevenly: 4,098 + 1,501 rows of 24 heads put 132 pairs of tiles on the busiest
+// of 148 CTAs, with a mean of 100. Heads of one block are neighbours, so that a group's K and V
+// come from L2.
 //
 // What bounds it: a pair of 128 x 128 tiles is 2,048 cycles of products and takes about 3,200; the
 // rest is the product warp's own time between them (a wait that finds its barrier done still
 // costs about 110 cycles) and the softmax, whose two sides share the special-function units.
-// Measured on one B200 (1.7 to 1.8 GHz under this load): 8,192 rows of 24 heads, all seen, 724 us
-// (1,140 TFLOP/s, 0.68 of the measured bf16 GEMM peak, 0.79 in the CTAs that are busy to the
-// end); 777..16,384 tokens causal 1.47 ms (1,210 TFLOP/s, 0.72); two prompts of 1,024 tokens 29 us,
-// where starting up (4 us to the first scores) and the longest unit (8 tiles) count.
+// Measured on one B200, captured, call after call (1.6 to 1.8 GHz under this load): 8,192 rows of 24
+// heads, all seen, 750 us (1,100 TFLOP/s, 0.65 of the measured bf16 GEMM peak, 0.75 in the CTAs that
+// are busy to the end); 777..16,384 tokens causal 1,630 us (1,090 TFLOP/s, 0.65); 4,098 + 1,501 rows,
+// all seen, 253 us. Two prompts of 1,024 tokens 30 us: the first weights are there after 6.6, a pair
+// of tiles of a first unit takes 2.4 (the first and the last of a side are masked, the last one's
+// values are cleaned before its softmax), an output 1.4, a quarter of the CTAs have a second unit
+// and the last of them ends at 25, 7.5 pairs in all; the rest passes between the calls.
 #include <algorithm>
 #include <atomic>
 #include <cmath>

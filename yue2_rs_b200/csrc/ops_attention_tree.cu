@@ -15,12 +15,14 @@
 //
 // A CTA is ten warps as in attention_packed: softmax of the sides, products, page loads (TMA).
 //
-// Measured on one B200, captured: trees of 64 and 48 nodes over 24,512 and 20,001 positions (24 / 8
-// heads of 128) 63 us against 28 us for the bytes alone; about 6 us pass before the first
-// weights (shares, page table, first tiles), a tile then takes 1.9 us (two sides of
-// products and softmax; the bytes alone 1.5), the partial results 3 and the merge 4. A batch of eight
-// trees at 63..8,191 positions 44 us against 18; one token of two sequences at 1,030
-// positions 15 us, all of it latency.
+// Measured on one B200, captured; the parts with timers in a copy. Trees of 64 and 48 nodes over
+// 24,512 and 20,001 positions (24 / 8 heads of 128) 60 us against 28 us for the bytes alone: the first
+// weights are there after 6.6 (shares 2.4, page table and first tiles 2.6, softmax 1.6), each of 17
+// more tiles takes 2.0 (two sides of products and softmax; the bytes alone 1.5), the output or
+// partial results 3.1, and the last CTA ends at 50; the other 10 are the launches and the merge. A
+// batch of eight trees at 63..8,191 positions 42 us against 18: 6.3, nine tiles of 1.9, 3, the last CTA
+// at 35, then 7. One token of two sequences at 1,030 positions 14.6 us, all of it latency: 6.3 to
+// the first weights, 9.7 for the last CTA, then 5.
 #include <algorithm>
 #include <atomic>
 #include <cmath>

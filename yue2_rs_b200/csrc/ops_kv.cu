@@ -3,10 +3,11 @@
 // written once); a page is [layers][K|V][kv] blocks of [64 positions][dim], so a position is
 // layers * 2 * kv separate runs of dim * 2 bytes.
 // Measured on one B200, captured, against the 6,544 GB/s of a plain copy: append of 8,192 rows of
-// 40 heads of 128 with packed K out 32 us (5.8 TB/s), two rows 2.3 us; the tails of 8 pages in 28
-// layers (58 MB) 11.3 us; accepting 8 of 64 nodes of 16 trees (29 MB in runs of 256 bytes)
-// 9.7 us, mostly the chain of list, table and row; evicting 4,001 of 8,192 positions (918 MB)
-// 147 us (6.2 TB/s).
+// 40 heads of 128 with packed K out 32 us (5.8 TB/s), two rows of 12 heads 2.2 us; the tails of 8
+// pages in 28 layers (58 MB) 11.6 us; accepting 8 of 64 nodes of 16 trees (29 MB in runs of 256
+// bytes) 9.8 us: the chain of list, table and row, then three blocks of a warp one after the
+// other with half of its row places empty; evicting 4,001 of 8,192 positions (918 MB) 147 us
+// (6.2 TB/s).
 #include <algorithm>
 #include <string>
 
