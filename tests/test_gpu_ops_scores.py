@@ -282,3 +282,34 @@ def test_tree_small_weights_in_half_precision(ops, rows, dim):
     ops.check_status()
     want, tol = small_tolerance(q[:rows], k, v)
     close(got[:, 0], want, tol)
+
+
+@pytest.mark.parametrize("at", [5, 130, 401, 2000])
+def test_infinitely_high_scores_make_their_rows_nan(ops, at):
+    # inf - inf in the row's own maximum; rows and sequences that do not see the key stay as they were
+    n, dim = 2500, 128
+    q, k, v = rows_of(n + 50, 2, dim, torch.bfloat16, 1), randn((n + 50, 2, dim), torch.bfloat16, 2), randn((n + 50, 2, dim), torch.bfloat16, 3)
+    cu = offsets([n, 50])
+    rng = random.Random(5)
+    pages, table = make_pages(rng, [n, 50])
+    data = torch.zeros((pages, 1, 2, 2, 64, dim), dtype=torch.bfloat16, device=DEV)
+
+    def both():
+        for s, (a, m) in enumerate(((0, n), (n, 50))):
+            pos = torch.arange(m, device=DEV)
+            page = ints(table[s]).long()[pos // 64]
+            data[page, 0, 0, :, pos % 64], data[page, 0, 1, :, pos % 64] = k[a:a + m], v[a:a + m]
+        tree = ops.attention_tree(q[:7], ops.KvPool(data), 0, ints(table), ints([n - 3, 46]), offsets([3, 4]))
+        out = ops.attention_packed(q, k, v, cu), ops.attention_packed(q, k, v, cu, causal=False), tree
+        ops.check_status()
+        return out
+
+    clean = both()
+    k[at, 1, C] = math.inf
+    got = both()
+    hit = torch.zeros_like(got[0], dtype=torch.bool)
+    hit[at:n, 1] = True
+    assert torch.isnan(got[0][hit]).all() and torch.equal(got[0][~hit], clean[0][~hit])
+    hit[:n, 1] = True
+    assert torch.isnan(got[1][hit]).all() and torch.equal(got[1][~hit], clean[1][~hit])
+    assert torch.isnan(got[2][:3, 1]).all() and torch.equal(got[2][:, 0], clean[2][:, 0]) and torch.equal(got[2][3:], clean[2][3:])
