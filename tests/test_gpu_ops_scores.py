@@ -218,6 +218,13 @@ def test_tree_keys_at_the_lowest_value(ops, nodes, scale, value):
     check_tree(ops, [700, 6000], [nodes, 2], lambda s, n: range(300), torch.bfloat16, 128, scale=scale, value=value)
 
 
+@pytest.mark.parametrize("ctx,dropped", [(9000, 4000), (700, 300), (24000, 20000)])
+def test_tree_keys_without_a_share_add_nothing(ops, ctx, dropped):
+    # scores so low that their weights are 0 beside the others', values of 2^110: in items that are cut,
+    # whole shares of them
+    check_tree(ops, [ctx], [2], lambda s, n: range(dropped), torch.bfloat16, 128, value=-1.0e12, huge=2.0 ** 110)
+
+
 @pytest.mark.parametrize("dtype,mag", [(torch.bfloat16, 1.0e3), (torch.bfloat16, 1.0e5), (torch.bfloat16, 1.0e9), (torch.float16, 2.0e3)])
 @pytest.mark.parametrize("causal", [True, False])
 def test_packed_large_scores(ops, causal, dtype, mag):

@@ -616,9 +616,10 @@ __global__ void __launch_bounds__(kMergeThreads, 6) tree_merge_kernel(const Tree
     float f = 0.f;
     if (base + lane <= c1) {
       const float2 s = stats[slot(base + lane)];
-      // not below the smallest normal number, so that infinities stay what they are; a share in
-      // which the row saw nothing has none
-      f = s.x == -INFINITY ? 0.f : max3(ex2(apart(a.c, s.x, m)), 1.17549435e-38f, 0.f);
+      // not below the smallest positive number, so that infinities stay what they are (and sums of
+      // large values vanish: the smallest normal number left 2^-126 of them); a share in which the
+      // row saw nothing has none
+      f = s.x == -INFINITY ? 0.f : max3(ex2(apart(a.c, s.x, m)), 1.4e-45f, 0.f);
       l = fmaf(s.y, f, l);
     }
     const int n = min(32, c1 - base + 1);
