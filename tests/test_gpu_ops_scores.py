@@ -320,3 +320,37 @@ def test_infinitely_high_scores_make_their_rows_nan(ops, at):
     hit[:n, 1] = True
     assert torch.isnan(got[1][hit]).all() and torch.equal(got[1][~hit], clean[1][~hit])
     assert torch.isnan(got[2][:3, 1]).all() and torch.equal(got[2][:, 0], clean[2][:, 0]) and torch.equal(got[2][3:], clean[2][3:])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("base", [0, 2 ** 11, 2 ** 14, 2 ** 15, 2 ** 18, 2 ** 22])
+def test_weights_across_tiles_of_large_exact_scores(ops, base, dtype):
+    # integer scores that f32 holds exactly, far above the differences that make the weights; every
+    # tile raises the maximum by about what its predecessors' weights are scaled down for. The
+    # exponent's constant is off by 2^-12 at most (a factor of 2^(2^-12) < 1 + 2^-12 for a tile
+    # beside another), exp and the sums by 2^-20, each weight and the output by half a step.
+    n, dim, nodes = 900, 64, 5
+    q, k, v = (torch.zeros((n, 1, dim), dtype=dtype, device=DEV) for _ in range(3))
+    side = 2 ** (math.frexp(max(base, 1))[1] // 2)
+    q[..., 0], k[..., 0] = side, base // side
+    g = torch.Generator(device=DEV).manual_seed(1)
+    steps = torch.arange(n, device=DEV) // 128 * 50 + torch.randint(0, 50, (n,), generator=g, device=DEV)
+    q[..., 1], q[..., 2], k[:, 0, 1], k[:, 0, 2] = 16, 1, (steps // 16).to(dtype), (steps % 16).to(dtype)
+    v = randn((n, 1, dim), dtype, 3)
+    scale = 1 / 8
+    score = q[:, 0].double() @ k[:, 0].double().T
+    assert torch.equal(score, score.round()) and float(score.max()) < 2 ** 23
+    u = torch.finfo(dtype).eps / 2
+    pages, table = make_pages(random.Random(3), [n])
+    data = torch.zeros((pages, 1, 2, 1, 64, dim), dtype=dtype, device=DEV)
+    pos = torch.arange(n, device=DEV)
+    page = ints(table[0]).long()[pos // 64]
+    data[page, 0, 0, 0, pos % 64], data[page, 0, 1, 0, pos % 64] = k[:, 0], v[:, 0]
+    tree = ops.attention_tree(q[-nodes:], ops.KvPool(data), 0, ints(table), ints([n - nodes]), offsets([nodes]))
+    for causal, got in ((True, ops.attention_packed(q, k, v, offsets([n]))), (False, ops.attention_packed(q, k, v, offsets([n]), causal=False)), (True, tree)):
+        s = torch.where(sees(n, causal), score * scale, -math.inf)[-got.shape[0]:]
+        p = torch.softmax(s, 1)
+        want, size = p @ v[:, 0].double(), p @ v[:, 0].double().abs()
+        tol = u * want.abs() + (u + 2 * 2.0 ** -12 + 2.0 ** -20) * size + 2.0 ** -32 * v[:, 0].double().abs().sum(0)[None]
+        close(got[:, 0], want, tol, (base, causal))
+    ops.check_status()

@@ -24,8 +24,8 @@
 // rest is the product warp's own time between them (a wait that finds its barrier done still
 // costs about 110 cycles) and the softmax, whose two sides share the special-function units.
 // Measured on one B200, captured, call after call (1.6 to 1.8 GHz under this load): 8,192 rows of 24
-// heads, all seen, 750 us (1,100 TFLOP/s, 0.65 of the measured bf16 GEMM peak, 0.75 in the CTAs that
-// are busy to the end); 777..16,384 tokens causal 1,630 us (1,090 TFLOP/s, 0.65); 4,098 + 1,501 rows,
+// heads, all seen, 755 us (1,090 TFLOP/s, 0.65 of the measured bf16 GEMM peak, 0.75 in the CTAs that
+// are busy to the end); 777..16,384 tokens causal 1,640 us (1,090 TFLOP/s, 0.65); 4,098 + 1,501 rows,
 // all seen, 253 us. Two prompts of 1,024 tokens 30 us: the first weights are there after 6.6, a pair
 // of tiles of a first unit takes 2.4 (the first and the last of a side are masked, the last one's
 // values are cleaned before its softmax), an output 1.4, a quarter of the CTAs have a second unit

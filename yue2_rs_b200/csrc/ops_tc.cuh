@@ -260,10 +260,11 @@ Y2_DEV void move_max(uint32_t o_addr, float c, bool first, float mn, RowStats& s
 // 2^-25 of the largest, nothing was left). The division by l removes it. bf16 has f32's range.
 template <bool F16>
 constexpr float kLift = F16 ? 7.f : 0.f;
-// Whether c s - c m, one FMA, is the exponent of a score s. c m is rounded, so that all weights of the
-// row share a factor of up to 2^(c m 2^-24), which the division by l removes as long as it fits the
-// weights' type: below 2^20 it is at most 2^(1/16). An infinite or NaN m is out of range, too.
-Y2_DEV bool in_range(float c, float m) { return fabsf(c * m) < 0x1p20f; }
+// Whether c s - c m, one FMA, is the exponent of a score s. c m is rounded, so that all weights formed
+// relative to this m share a factor of up to 2^(c m 2^-24). The division by l removes it, except
+// beside tiles with another m: below 2^12 it is at most 2^(2^-12), a third of half a step of f16. An
+// infinite or NaN m is out of range, too.
+Y2_DEV bool in_range(float c, float m) { return fabsf(c * m) < 0x1p12f; }
 // The exponent of any row: (a s + b) k + kLift. An m of +inf or NaN makes the row NaN; an m of -inf
 // (no score above it yet) gives every weight 0.
 struct Exponent {
